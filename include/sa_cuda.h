@@ -339,6 +339,106 @@ int sa_attn_decode_noalloc(void* stream, int dtype, const void* q, const void* k
                            float scale, float* out);
 
 /* ======================================================================== */
+/* Attention over a paged KV cache (batches of sequences)                    */
+/* ======================================================================== */
+
+/*
+ * A cache for many sequences: pools of pages, and per sequence the pages that
+ * hold its rows.  These calls have no counterpart in the reference (its
+ * KVCache, kv_cache.h:24-70, is one contiguous tensor per layer at batch 1).
+ *
+ *   k_pages, v_pages  [n_pages, hkv, page_size, d], element type `dtype`,
+ *                     page_stride elements between pages (>= hkv * page_size *
+ *                     d, so K and V may be interleaved in one pool)
+ *   block_table       [n_seqs] rows of table_stride int32 (>= max_pages), in
+ *                     device memory: row r of sequence b lies in page
+ *                     block_table[b][r / page_size] at row r % page_size.
+ *                     Entries of pages that no query of the call sees are not
+ *                     read as pages and may hold anything (-1, a freed page)
+ *   kv_lens           [n_seqs] int32 in device memory: rows of each sequence,
+ *                     those appended for the call included (0: none)
+ *
+ * Rows of a sequence are finite numbers; what pages hold past kv_lens may be
+ * anything, NaN included.  Requirements: dtype SA_F32 or SA_BF16; d 64, 128
+ * or 256; page_size 16, 32, 64 or 128; hq / hkv 1..16 (1..8 at d = 256);
+ * pointers 16-byte aligned, strides multiples of 16 bytes; n_seqs at most
+ * SA_PAGED_MAX_SEQS.  q and out have the cache's element type; scale is
+ * positive and finite.  Device pointers only.
+ *
+ * A query at position p sees row j when j <= p and (window = 0, or
+ * j > p - window, or j < sinks): a sliding window of `window` rows, its own
+ * included, and the first `sinks` rows.  A query that sees nothing (an empty
+ * sequence) gets zeros.
+ *
+ * Everything is read on the device when the call runs, so a captured launch
+ * stays right as lengths and tables change.  A length that exceeds
+ * max_pages * page_size is cut, a page number outside the pool is not
+ * accessed (its rows' contribution is undefined), and sa_ctx_synchronize then
+ * returns SA_ERR_RANGE.
+ *
+ * Workspaces are the caller's (256-byte aligned device memory, contents
+ * arbitrary); calls that may run at the same time, captured ones included,
+ * need workspaces of their own.  Their sizes depend on the shapes in kv and on
+ * hq (and n_tokens), not on lengths.
+ */
+#define SA_PAGED_MAX_SEQS 65536
+typedef struct {
+    void* k_pages;
+    void* v_pages;
+    int dtype;
+    int n_pages, page_size, hkv, d;
+    long long page_stride;
+    const int* block_table;
+    long long table_stride;
+    int max_pages;
+    const int* kv_lens;
+    int n_seqs;
+} sa_paged_kv;
+
+/*
+ * Tables of rotary angles: cos_t, sin_t [n_pos, rotary_dim / 2] fp32 (device
+ * memory) of p * theta^(-2i / rotary_dim), the angles taken in 64 bits.
+ */
+int sa_rope_table(sa_ctx* ctx, int n_pos, int rotary_dim, double theta, float* cos_t, float* sin_t);
+
+/*
+ * Append new tokens to their sequences, rotating keys (and queries) by their
+ * positions on the way.
+ *   q [n_tokens, hq, d] (NULL: none), k, v [n_tokens, hkv, d], element type
+ *     x_dtype, token strides in elements (column slices of one projection
+ *     output are fine)
+ *   cu_q [n_seqs + 1] int32 (device): tokens cu_q[b] .. cu_q[b+1] - 1 are
+ *     sequence b's, its last ones: token t of n goes to row kv_lens[b] - n + t.
+ *     NULL: one token per sequence, token b to row kv_lens[b] - 1 (sequences
+ *     of length 0 are slots of a padded batch and are passed over).  Tokens
+ *     behind the last sequence are passed over.
+ *   cos_t, sin_t [n_pos, rotary_dim / 2] fp32 (both NULL: no rotation): the
+ *     angle of position pos0 + row.  pos0 is the length of a prefix that is
+ *     kept in other pages (0 otherwise).  rotary_dim is a multiple of 16, at
+ *     most d; elements past it are copied.  interleaved 0: element i turns
+ *     with i + rotary_dim / 2; 1: element 2i with 2i + 1.
+ *   q_out [n_tokens, hq, d], the cache's element type: the rotated queries
+ *     (may be q itself if the types agree).
+ * Arithmetic in fp32, one rounding to the cache's type.  A row outside the
+ * block table or the angle table is not written (SA_ERR_RANGE at
+ * sa_ctx_synchronize).
+ */
+int sa_paged_append(sa_ctx* ctx, const sa_paged_kv* kv, int x_dtype, const void* q, long long q_tok_stride,
+                    const void* k, long long k_tok_stride, const void* v, long long v_tok_stride, int n_tokens,
+                    int hq, const int* cu_q, int pos0, const float* cos_t, const float* sin_t, int n_pos,
+                    int rotary_dim, int interleaved, void* q_out, long long qo_tok_stride);
+
+/*
+ * One query token per sequence, at its last row: q, out [n_seqs, hq, d] with
+ * q_stride / o_stride elements between sequences.  Softmax and sums in fp32;
+ * bf16 products take the softmax weights in bf16 (as the output is).
+ */
+int sa_attn_paged_decode_workspace(sa_ctx* ctx, const sa_paged_kv* kv, int hq, size_t* bytes);
+int sa_attn_paged_decode(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_stride, int hq, int window,
+                         int sinks, float scale, void* out, long long o_stride, void* workspace,
+                         size_t workspace_bytes);
+
+/* ======================================================================== */
 /* Qwen3 forward                                                             */
 /* ======================================================================== */
 

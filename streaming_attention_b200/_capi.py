@@ -25,8 +25,22 @@ SA_BF16 = 1
 SA_HOST_PTRS = 1
 SA_KV_STATIC = 2
 
+SA_PAGED_MAX_SEQS = 65536
+
 _vp = C.c_void_p
 _fp = C.POINTER(C.c_float)
+
+
+
+class PagedKV(C.Structure):
+    """sa_paged_kv: a paged KV cache and its sequences."""
+    _fields_ = [("k_pages", _vp), ("v_pages", _vp), ("dtype", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("hkv", C.c_int), ("d", C.c_int), ("page_stride", C.c_longlong), ("block_table", _vp),
+                ("table_stride", C.c_longlong), ("max_pages", C.c_int), ("kv_lens", _vp), ("n_seqs", C.c_int)]
+
+
+_kvp = C.POINTER(PagedKV)
+_szp = C.POINTER(C.c_size_t)
 
 # (name, restype, argtypes) for every entry point of include/sa_cuda.h
 SIGNATURES = {
@@ -95,6 +109,13 @@ SIGNATURES = {
                                     C.c_int, C.c_int, C.c_int, C.c_float, _vp, _vp, _vp, C.c_uint]),
     "sa_attn_decode_noalloc": (C.c_int, [_vp, C.c_int, _vp, _vp, _vp, C.c_longlong, C.c_int,
                                          C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, _vp]),
+    "sa_rope_table": (C.c_int, [_vp, C.c_int, C.c_int, C.c_double, _vp, _vp]),
+    "sa_paged_append": (C.c_int, [_vp, _kvp, C.c_int, _vp, C.c_longlong, _vp, C.c_longlong, _vp, C.c_longlong,
+                                  C.c_int, C.c_int, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, _vp,
+                                  C.c_longlong]),
+    "sa_attn_paged_decode_workspace": (C.c_int, [_vp, _kvp, C.c_int, _szp]),
+    "sa_attn_paged_decode": (C.c_int, [_vp, _kvp, _vp, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float, _vp,
+                                       C.c_longlong, _vp, C.c_size_t]),
 }
 
 

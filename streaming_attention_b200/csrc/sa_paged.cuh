@@ -1,0 +1,138 @@
+// sa_paged.cuh -- what the operators over a paged KV cache share: the view of
+// the cache that kernels take, the visible rows of a query under a sliding
+// window with first tokens that stay visible, and the host-side checks.
+#pragma once
+#include <cuda.h>
+#include <cstdint>
+
+#include "sa_internal.h"
+#include "sa_paged_plan.h"
+#include "sa_ptx.cuh"
+#include "sa_tc.cuh"
+
+namespace sa {
+namespace pg {
+
+constexpr int MAX_GROUP = 16;      // largest hq / hkv
+
+// The cache as kernels see it: pages of [hkv][page][d] elements.
+struct Cache {
+    unsigned char* k;
+    unsigned char* v;
+    const int* table;          // [n_seqs] rows of table_stride entries
+    const int* kv_lens;        // [n_seqs]
+    long long page_stride;     // elements between pages
+    long long table_stride;
+    int n_pages, page_log2, hkv, n_seqs, max_pages;
+    int* status;
+};
+
+// Rows of sequence b, within [0, max_pages * page]; a length past what the
+// block table can hold is reported and cut.
+__device__ __forceinline__ int seq_len(const Cache& c, int b) {
+    const int n = c.kv_lens[b], cut = cut_len(n, c.max_pages, c.page_log2);
+    if (cut < n) atomicExch(c.status, SA_STATUS_BAD_INDEX);
+    return cut;
+}
+
+// The page that a block-table entry names, or -1 (reported) if it is none of
+// the pool's.
+__device__ __forceinline__ int checked_page(const Cache& c, int entry) {
+    if (page_ok(entry, c.n_pages)) return entry;
+    atomicExch(c.status, SA_STATUS_BAD_INDEX);
+    return -1;
+}
+
+// ---- host ------------------------------------------------------------------
+inline int log2_exact(int x) {
+    int l = 0;
+    while ((1 << l) < x) ++l;
+    return (1 << l) == x ? l : -1;
+}
+
+// Checks of a cache description that every entry point makes.
+inline int check_cache(const char* fn, const sa_paged_kv* kv) {
+    SA_CHECK_ARG(kv != nullptr, "%s: kv is NULL", fn);
+    SA_CHECK_ARG(kv->dtype == SA_F32 || kv->dtype == SA_BF16, "%s: dtype %d (want SA_F32 or SA_BF16)", fn, kv->dtype);
+    SA_CHECK_ARG(kv->k_pages && kv->v_pages, "%s: null k_pages/v_pages", fn);
+    SA_CHECK_ARG(kv->d == 64 || kv->d == 128 || kv->d == 256, "%s: d = %d (supported: 64, 128, 256)", fn, kv->d);
+    SA_CHECK_ARG(kv->page_size == 16 || kv->page_size == 32 || kv->page_size == 64 || kv->page_size == 128,
+                 "%s: page_size = %d (supported: 16, 32, 64, 128)", fn, kv->page_size);
+    SA_CHECK_ARG(kv->hkv >= 1 && kv->hkv <= SA_MAX_KV_HEADS, "%s: hkv = %d (1..%d)", fn, kv->hkv, SA_MAX_KV_HEADS);
+    SA_CHECK_ARG(kv->n_pages >= 1, "%s: n_pages = %d", fn, kv->n_pages);
+    SA_CHECK_ARG(kv->n_seqs >= 0 && kv->n_seqs <= SA_PAGED_MAX_SEQS, "%s: n_seqs = %d (0..%d)", fn, kv->n_seqs,
+                 SA_PAGED_MAX_SEQS);
+    SA_CHECK_ARG(kv->max_pages >= 0 && kv->table_stride >= kv->max_pages, "%s: max_pages %d, table_stride %lld", fn,
+                 kv->max_pages, kv->table_stride);
+    SA_CHECK_ARG((long long)kv->max_pages * kv->page_size <= 0x7ffffe00LL,
+                 "%s: %d pages of %d rows per sequence exceed the 2^31 positions of a sequence", fn, kv->max_pages,
+                 kv->page_size);
+    SA_CHECK_ARG(kv->n_seqs == 0 || (kv->kv_lens && (kv->max_pages == 0 || kv->block_table)),
+                 "%s: null block_table/kv_lens", fn);
+    const int e = kv->dtype == SA_F32 ? 4 : 2;
+    SA_CHECK_ARG(kv->page_stride >= (long long)kv->hkv * kv->page_size * kv->d && kv->page_stride * e % 16 == 0,
+                 "%s: page_stride %lld (at least hkv * page_size * d = %lld elements, a multiple of 16 bytes)", fn,
+                 kv->page_stride, (long long)kv->hkv * kv->page_size * kv->d);
+    SA_CHECK_ARG((((uintptr_t)kv->k_pages | (uintptr_t)kv->v_pages) & 15) == 0,
+                 "%s: k_pages/v_pages not 16-byte aligned", fn);
+    return SA_OK;
+}
+
+inline int check_heads(const char* fn, const sa_paged_kv* kv, int hq) {
+    SA_CHECK_ARG(hq >= 1 && hq % kv->hkv == 0 && hq / kv->hkv <= MAX_GROUP, "%s: hq = %d, hkv = %d (hq/hkv 1..%d)", fn,
+                 hq, kv->hkv, MAX_GROUP);
+    SA_CHECK_ARG(kv->d < 256 || hq / kv->hkv <= 8, "%s: hq/hkv = %d at d = 256 (at most 8)", fn, hq / kv->hkv);
+    return SA_OK;
+}
+
+inline int check_scale(const char* fn, float scale) {
+    SA_CHECK_ARG(scale > 0.f && scale <= 3.0e38f, "%s: scale = %g (want a positive finite number)", fn, (double)scale);
+    return SA_OK;
+}
+
+// A row tensor's token stride and address.
+inline int check_rows(const char* fn, const char* what, const void* p, long long stride, long long width, int e) {
+    SA_CHECK_ARG(p != nullptr && ((uintptr_t)p & 15) == 0, "%s: %s is NULL or not 16-byte aligned", fn, what);
+    SA_CHECK_ARG(stride >= width && stride * e % 16 == 0,
+                 "%s: %s token stride %lld (at least %lld elements, a multiple of 16 bytes)", fn, what, stride, width);
+    return SA_OK;
+}
+
+inline Cache make_cache(const sa_ctx* ctx, const sa_paged_kv* kv) {
+    Cache c;
+    c.k = static_cast<unsigned char*>(kv->k_pages);
+    c.v = static_cast<unsigned char*>(kv->v_pages);
+    c.table = kv->block_table;
+    c.kv_lens = kv->kv_lens;
+    c.page_stride = kv->page_stride;
+    c.table_stride = kv->table_stride;
+    c.n_pages = kv->n_pages;
+    c.page_log2 = log2_exact(kv->page_size);
+    c.hkv = kv->hkv;
+    c.n_seqs = kv->n_seqs;
+    c.max_pages = kv->max_pages;
+    c.status = ctx->status;
+    return c;
+}
+
+// 3-D bf16 tensor map (d, rows of a page, pages) over a pool, box 64 columns x
+// box_rows rows x 1 page, 128-byte swizzle.  A page coordinate outside the
+// pool reads zeros.
+inline int make_page_tmap(CUtensorMap* map, const void* pages, const sa_paged_kv* kv, int box_rows) {
+    const uint64_t n[3] = {(uint64_t)kv->d, (uint64_t)kv->hkv * kv->page_size, (uint64_t)kv->n_pages};
+    const uint64_t stride[2] = {(uint64_t)kv->d, (uint64_t)kv->page_stride};
+    const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
+    return make_tmap_3d_bf16(map, pages, n, stride, box);
+}
+// 3-D bf16 tensor map (d, heads, tokens) over query rows, box 64 columns x
+// `group` heads x `toks` tokens, 128-byte swizzle: rows land token after token.
+inline int make_query_tmap(CUtensorMap* map, const void* q, int d, int hq, int n_tokens, long long tok_stride, int group,
+                           int toks) {
+    const uint64_t n[3] = {(uint64_t)d, (uint64_t)hq, (uint64_t)n_tokens};
+    const uint64_t stride[2] = {(uint64_t)d, (uint64_t)tok_stride};
+    const uint32_t box[3] = {64, (uint32_t)group, (uint32_t)toks};
+    return make_tmap_3d_bf16(map, q, n, stride, box);
+}
+
+}  // namespace pg
+}  // namespace sa

@@ -1,0 +1,27 @@
+// sa_paged_decode.h -- the paged decode's launch and workspace, for the
+// shared-prefix decode that runs it on the sequences' own rows.
+#pragma once
+#include "sa_internal.h"
+
+namespace sa {
+namespace pg {
+
+// Shares of (sequence, KV head) pairs that several CTAs hold.  States are rows
+// of d + 2 floats: the unnormalised O, then m (log2 domain) and l.
+struct DecodeWs {
+    float* slots;     // [grid][2][G]: the first and the last pair of a CTA
+    int4* head;       // [grid]: first CTA, last CTA, first CTA's slot, pair; first CTA -1: nothing to join
+    int4* pair;       // [n_seqs * hkv] the same by pair (first CTA -1: the state is whole), with `state`
+    float* state;     // [n_seqs][hq]
+    int d, out_elt;
+};
+
+int decode_grid(const sa_ctx* ctx, const sa_paged_kv* kv, int hq);
+// Lays the workspace out at `base` (may be null) and returns its size.
+size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool to_state, void* base, DecodeWs* ws);
+// to_state: every pair's state goes to ws (pair, state, slots) and `out` is not written.
+int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_stride, int hq, int window, int sinks,
+                  float scale, void* out, long long o_stride, bool to_state, const DecodeWs& ws);
+
+}  // namespace pg
+}  // namespace sa

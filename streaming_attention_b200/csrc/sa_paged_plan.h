@@ -1,0 +1,66 @@
+// sa_paged_plan.h -- which rows and pages the operators over a paged KV cache
+// touch, and how a batch's tiles are shared out, as plain arithmetic: included
+// by the kernels and compiled with g++ by a CPU test that enumerates it.
+#pragma once
+
+#ifndef __CUDACC__
+#define SA_HD
+#else
+#define SA_HD __host__ __device__
+#endif
+
+namespace sa {
+namespace pg {
+
+// Rows of a sequence that the block table can hold.
+SA_HD inline int cut_len(int len, int max_pages, int page_log2) {
+    const long long cap = (long long)max_pages << page_log2;
+    return len < 0 ? 0 : (len > cap ? (int)cap : len);
+}
+SA_HD inline bool page_ok(int entry, int n_pages) { return (unsigned)entry < (unsigned)n_pages; }
+
+// A query at position p sees row j when j <= p and (no window, or
+// j > p - window, or j < sinks).  The first row of its window:
+SA_HD inline int window_lo(int p, int window) { return (window > 0 && p >= window) ? p - window + 1 : 0; }
+
+// The rows that ONE query over `len` rows sees, cut into tiles of `tk` rows
+// that start at multiples of tk: tiles [0, ta) hold the first tokens, then
+// tiles tb0.. hold the window; a tile that holds both is counted once.
+struct Tiles {
+    int len, lo, sinks, ta, tb0, n;
+    SA_HD inline int row0(int i, int tk) const { return (i < ta ? i : i - ta + tb0) * tk; }
+    SA_HD inline bool sees(int row) const { return row < len && (row >= lo || row < sinks); }
+    // some row of [r0, r0 + n) is seen / every one is
+    SA_HD inline bool any(int r0, int rows) const { return r0 < len && (r0 + rows > lo || r0 < sinks); }
+    SA_HD inline bool all(int r0, int rows) const { return r0 + rows <= len && (r0 >= lo || r0 + rows <= sinks); }
+};
+SA_HD inline Tiles make_tiles(int len, int window, int sinks, int tk) {
+    Tiles t;
+    t.len = len;
+    t.lo = window_lo(len - 1, window);
+    if (sinks >= t.lo) t.lo = 0;                 // the first tokens reach the window: all rows are seen
+    t.sinks = sinks < t.lo ? sinks : t.lo;
+    t.ta = (t.sinks + tk - 1) / tk;
+    t.tb0 = t.lo / tk > t.ta ? t.lo / tk : t.ta;
+    const int tb1 = (int)(((long long)len + tk - 1) / tk);
+    t.n = t.ta + (tb1 > t.tb0 ? tb1 - t.tb0 : 0);
+    return t;
+}
+
+// A list of `total` tiles shared out over n CTAs (n <= total): the first tile
+// of CTA c, and the CTA that a tile falls to.
+SA_HD inline long long share_first(long long c, long long total, long long n) { return c * total / n; }
+SA_HD inline int share_of(long long tile, long long total, long long n) {
+    return (int)(((tile + 1) * n - 1) / total);
+}
+
+// The row of token t (of n) of a sequence of `len` rows, -1 if the cache has
+// no such row or the angle table no such position.
+SA_HD inline long long append_row(int len, int n, int t, int max_pages, int page_log2, long long pos0, long long n_pos) {
+    const long long at = (long long)len - n + t;
+    if (at < 0 || (at >> page_log2) >= max_pages || pos0 + at >= n_pos) return -1;
+    return at;
+}
+
+}  // namespace pg
+}  // namespace sa

@@ -47,6 +47,28 @@ int make_tmap_2d_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_
     return SA_OK;
 }
 
+// 3-D bf16 tensor map over [dims2][dims1][dims0] elements with element strides
+// between the outer coordinates, 128-byte swizzle, zeros outside.
+int make_tmap_3d_bf16(CUtensorMap* map, const void* base, const uint64_t (&n)[3], const uint64_t (&stride)[2],
+                      const uint32_t (&box)[3]) {
+    int rc = get_encode();
+    if (rc) return rc;
+    SA_CHECK_ARG(((uintptr_t)base & 15) == 0 && stride[0] * 2 % 16 == 0 && stride[1] * 2 % 16 == 0,
+                 "tensor map base or strides not 16-byte aligned");
+    const cuuint64_t dims[3] = {n[0], n[1], n[2]};
+    const cuuint64_t strides[2] = {stride[0] * 2, stride[1] * 2};
+    const cuuint32_t bx[3] = {box[0], box[1], box[2]};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, bx, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(SA_ERR_ARG, "cuTensorMapEncodeTiled failed (%d): [%llu, %llu, %llu] strides %llu, %llu", (int)r,
+                         (unsigned long long)n[2], (unsigned long long)n[1], (unsigned long long)n[0],
+                         (unsigned long long)stride[1], (unsigned long long)stride[0]);
+    return SA_OK;
+}
+
 // 2-D fp32 tensor map over a row-major [rows, cols] block (row stride
 // row_stride_elems), box [box_rows, 32 columns], 128-byte swizzle: KV-cache
 // rows for the prompt attention (16-byte chunk q of row r lands at chunk
