@@ -438,6 +438,32 @@ int sa_attn_paged_decode(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long
                          int sinks, float scale, void* out, long long o_stride, void* workspace,
                          size_t workspace_bytes);
 
+/*
+ * A ragged batch of prompt chunks: q, out [n_tokens, hq, d] (token strides in
+ * elements), tokens cu_q[b] .. cu_q[b+1] - 1 the last ones of sequence b
+ * (token t of n at position kv_lens[b] - n + t), whose keys and values are in
+ * the pages.  Causal, with the window above.  bf16 on the tensor cores
+ * (softmax weights in bf16, sums in fp32), fp32 on CUDA cores.  d 64 or 128.
+ * Rows behind the last sequence are left as they were.
+ */
+int sa_attn_paged_prefill(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_tok_stride, int n_tokens,
+                          int hq, const int* cu_q, int window, int sinks, float scale, void* out,
+                          long long o_tok_stride);
+
+/*
+ * One query token per sequence, over a prefix that all sequences share and
+ * then the sequence's own rows: q, out [n_seqs, hq, d].  prefix_table lists
+ * the pages of the prefix_len shared rows (device memory, ceil(prefix_len /
+ * page_size) entries); kv's block table and lengths are those of the own rows
+ * alone (a length may be 0).  The prefix is read once for the whole batch.
+ * d 64 or 128.
+ */
+int sa_attn_paged_decode_prefix_workspace(sa_ctx* ctx, const sa_paged_kv* kv, int hq, int prefix_len,
+                                          size_t* bytes);
+int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const int* prefix_table, int prefix_len,
+                                const void* q, long long q_stride, int hq, float scale, void* out,
+                                long long o_stride, void* workspace, size_t workspace_bytes);
+
 /* ======================================================================== */
 /* Qwen3 forward                                                             */
 /* ======================================================================== */

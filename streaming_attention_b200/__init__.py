@@ -28,12 +28,18 @@ from .attention import (  # noqa: F401
     streaming_attention_mpi_cuda,
 )
 
-from .paged import attn_paged_decode, paged_append, rope_table  # noqa: F401
+from .paged import (  # noqa: F401
+    attn_paged_decode,
+    attn_paged_decode_prefix,
+    attn_paged_prefill,
+    paged_append,
+    rope_table,
+)
 from .qwen3 import QWEN3_0_6B, Qwen3, Qwen3Config  # noqa: F401
 
 __all__ = [
     "Context", "SAError", "lib", "LIB_PATH", "SA_F32", "SA_BF16", "SA_HOST_PTRS",
     "attn_decode", "attn_decode_partial", "attn_decode_step", "attn_merge", "attn_prefill", "attn_prompt_f32", "streaming_attention_cuda",
     "naive_attention_cuda", "streaming_attention_mpi_cuda", "Qwen3", "Qwen3Config", "QWEN3_0_6B",
-    "paged_append", "rope_table", "attn_paged_decode",
+    "paged_append", "rope_table", "attn_paged_decode", "attn_paged_prefill", "attn_paged_decode_prefix",
 ]

@@ -116,6 +116,11 @@ SIGNATURES = {
     "sa_attn_paged_decode_workspace": (C.c_int, [_vp, _kvp, C.c_int, _szp]),
     "sa_attn_paged_decode": (C.c_int, [_vp, _kvp, _vp, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_float, _vp,
                                        C.c_longlong, _vp, C.c_size_t]),
+    "sa_attn_paged_prefill": (C.c_int, [_vp, _kvp, _vp, C.c_longlong, C.c_int, C.c_int, _vp, C.c_int, C.c_int,
+                                        C.c_float, _vp, C.c_longlong]),
+    "sa_attn_paged_decode_prefix_workspace": (C.c_int, [_vp, _kvp, C.c_int, C.c_int, _szp]),
+    "sa_attn_paged_decode_prefix": (C.c_int, [_vp, _kvp, _vp, C.c_int, _vp, C.c_longlong, C.c_int, C.c_float, _vp,
+                                              C.c_longlong, _vp, C.c_size_t]),
 }
 
 

@@ -43,6 +43,65 @@ __device__ __forceinline__ int checked_page(const Cache& c, int entry) {
     return -1;
 }
 
+// The tokens of a ragged batch cut into units of up to `per` tokens of one
+// sequence, numbered over the batch.
+struct SeqUnit {
+    int b, unit;            // sequence, unit of it
+    int first, tokens;      // the sequence's first row in the token tensors, its tokens
+};
+// Tokens of sequence b; a range outside the token tensors is reported and
+// counts as none.
+__device__ __forceinline__ int seq_tokens(const Cache& c, const int* cu_q, int n_tok, int b, int* first) {
+    const int c0 = cu_q[b], c1 = cu_q[b + 1];
+    *first = c0;
+    if (c0 < 0 || c1 > n_tok || c1 < c0) {
+        atomicExch(c.status, SA_STATUS_BAD_INDEX);
+        return 0;
+    }
+    return c1 - c0;
+}
+// Unit total - 1 - back of the batch, by the whole block (scan: THREADS / 32
+// ints); false when there is none.
+template <int THREADS>
+__device__ bool find_seq_unit(const Cache& c, const int* cu_q, int n_tok, int per, int back, SeqUnit* s, int* scan) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int run = (c.n_seqs + THREADS - 1) / THREADS;
+    const int b0 = min(c.n_seqs, tid * run), b1 = min(c.n_seqs, b0 + run);
+    int first, mine = 0;
+    for (int b = b0; b < b1; ++b) mine += (seq_tokens(c, cu_q, n_tok, b, &first) + per - 1) / per;
+    int inc = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, inc, off);
+        if (lane >= off) inc += up;
+    }
+    if (lane == 31) scan[warp] = inc;
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) before += scan[w];
+        total += scan[w];
+    }
+    const int want = total - 1 - back;
+    if (want < 0) return false;
+    int at = before + inc - mine;
+    if (want >= at && want < at + mine)
+        for (int b = b0; b < b1; ++b) {
+            const int n = seq_tokens(c, cu_q, n_tok, b, &first), u = (n + per - 1) / per;
+            if (want < at + u) {
+                s->b = b;
+                s->unit = want - at;
+                s->first = first;
+                s->tokens = n;
+                break;
+            }
+            at += u;
+        }
+    __syncthreads();
+    return true;
+}
+
 // ---- host ------------------------------------------------------------------
 inline int log2_exact(int x) {
     int l = 0;

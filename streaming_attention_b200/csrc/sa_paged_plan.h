@@ -47,6 +47,32 @@ SA_HD inline Tiles make_tiles(int len, int window, int sinks, int tk) {
     return t;
 }
 
+// The same for the query rows of one CTA of the tensor-core kernel: two slots
+// of consecutive queries, the first query at position p0 and the slots' last
+// ones at last[0] and last[1] (-1: the slot sees nothing).  Tiles hold every
+// row that some query sees; slot x takes the first n[x] of them.
+struct UnitTiles {
+    Tiles t;          // t.n = max of n[]
+    int n[2];
+};
+SA_HD inline UnitTiles make_unit(int p0, int last0, int last1, int window, int sinks, int tk) {
+    UnitTiles u;
+    const int last = last0 > last1 ? last0 : last1;
+    u.t.len = last < 0 ? 0 : last + 1;
+    u.t.lo = window_lo(p0 < 0 ? 0 : p0, window);
+    if (sinks >= u.t.lo) u.t.lo = 0;
+    u.t.sinks = sinks < u.t.lo ? sinks : u.t.lo;
+    u.t.ta = (u.t.sinks + tk - 1) / tk;
+    u.t.tb0 = u.t.lo / tk > u.t.ta ? u.t.lo / tk : u.t.ta;
+    for (int x = 0; x < 2; ++x) {
+        const int l = x ? last1 : last0;
+        const int end = l < 0 ? 0 : l / tk + 1;
+        u.n[x] = l < 0 ? 0 : u.t.ta + (end > u.t.tb0 ? end - u.t.tb0 : 0);
+    }
+    u.t.n = u.n[0] > u.n[1] ? u.n[0] : u.n[1];
+    return u;
+}
+
 // A list of `total` tiles shared out over n CTAs (n <= total): the first tile
 // of CTA c, and the CTA that a tile falls to.
 SA_HD inline long long share_first(long long c, long long total, long long n) { return c * total / n; }

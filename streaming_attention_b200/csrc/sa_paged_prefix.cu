@@ -1,0 +1,220 @@
+// sa_paged_prefix.cu -- the C entries of the paged prefill and of the decode
+// behind a shared prefix, and the join of the latter's states.
+//
+// softmax over [prefix rows, own rows] from states (m, l, O) of parts of them:
+//   m = max m_i,  l = sum 2^(m_i - m) l_i,  O = sum 2^(m_i - m) O_i,  out = O / l.
+// The prefix is read once for all sequences: its query rows are the B x G
+// (sequence, head) pairs of a KV head, a matrix product with B G rows where a
+// decode per sequence would read the prefix B times.
+#include <cuda_bf16.h>
+#include <algorithm>
+
+#include "sa_paged.cuh"
+#include "sa_paged_decode.h"
+#include "sa_paged_f32.h"
+#include "sa_paged_tc.h"
+
+namespace sa {
+namespace pg {
+
+constexpr int JT = 256;
+
+struct JoinArgs {
+    Cache c;
+    DecodeWs ws;
+    void* out;
+    long long o_stride;
+    int hq, G;
+    int n_split, alt_from;       // rows of sequences >= alt_from have 2 n_split parts, the others n_split
+    const float* part_o;
+    const float* part_ml;
+};
+
+struct Acc {
+    float m, l, o[4];
+    __device__ __forceinline__ void add(float m2, float l2, float4 o2) {
+        const float M = fmaxf(m, m2);
+        const float wa = m == -INFINITY ? 0.f : ex2(m - M), wb = m2 == -INFINITY ? 0.f : ex2(m2 - M);
+        m = M;
+        l = l * wa + l2 * wb;
+        o[0] = o[0] * wa + o2.x * wb;
+        o[1] = o[1] * wa + o2.y * wb;
+        o[2] = o[2] * wa + o2.z * wb;
+        o[3] = o[3] * wa + o2.w * wb;
+    }
+};
+
+// D / 4 threads per (sequence, query head).
+template <typename OT, int D>
+__global__ void __launch_bounds__(JT) prefix_join_kernel(const __grid_constant__ JoinArgs a) {
+    pdl_wait();
+    constexpr int TPR = D / 4;
+    const long long row = (long long)blockIdx.x * (JT / TPR) + threadIdx.x / TPR;
+    const int c4 = (threadIdx.x % TPR) * 4;
+    const long long rows = (long long)a.c.n_seqs * a.hq;
+    if (row >= rows) return;
+    const int b = (int)(row / a.hq), h = (int)(row - (long long)b * a.hq), kvh = h / a.G, g = h - kvh * a.G;
+    Acc s;
+    s.m = -INFINITY;
+    s.l = s.o[0] = s.o[1] = s.o[2] = s.o[3] = 0.f;
+    const int parts = b >= a.alt_from ? 2 * a.n_split : a.n_split;
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+        const long long at = (long long)p * rows + row;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
+        // an empty part has no O
+        if (ml.x != -INFINITY) s.add(ml.x, ml.y, *reinterpret_cast<const float4*>(a.part_o + at * D + c4));
+    }
+    if (seq_len(a.c, b) > 0) {
+        const int4 rec = a.ws.pair[b * a.c.hkv + kvh];
+        const int n = rec.x < 0 ? 1 : rec.y - rec.x + 1;
+        for (int i = 0; i < n; ++i) {
+            const float* st = rec.x < 0 ? a.ws.state + row * (D + 2)
+                                        : a.ws.slots + ((2LL * (rec.x + i) + (i == 0 ? rec.z : 0)) * a.G + g) * (D + 2);
+            const float2 u = *reinterpret_cast<const float2*>(st + c4), w = *reinterpret_cast<const float2*>(st + c4 + 2);
+            s.add(st[D], st[D + 1], make_float4(u.x, u.y, w.x, w.y));
+        }
+    }
+    const bool failed = *reinterpret_cast<volatile int*>(a.c.status) == SA_STATUS_TIMEOUT;
+    const float f = failed ? nanf("") : (s.l > 0.f ? 1.f / s.l : 0.f);
+    const long long at = (long long)b * a.o_stride + (long long)h * D + c4;
+    if constexpr (sizeof(OT) == 4) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) =
+            make_float4(s.o[0] * f, s.o[1] * f, s.o[2] * f, s.o[3] * f);
+    } else {
+        const __nv_bfloat162 u = __floats2bfloat162_rn(s.o[0] * f, s.o[1] * f);
+        const __nv_bfloat162 w = __floats2bfloat162_rn(s.o[2] * f, s.o[3] * f);
+        uint2 x;
+        x.x = *reinterpret_cast<const uint32_t*>(&u);
+        x.y = *reinterpret_cast<const uint32_t*>(&w);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = x;
+    }
+}
+
+struct PrefixWs {
+    DecodeWs own;
+    float *part_o, *part_ml;
+    int n_split;
+};
+static size_t prefix_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, int prefix_len, void* base,
+                               PrefixWs* ws) {
+    PrefixWs w = {};
+    size_t at = align_up(decode_ws_layout(ctx, kv, hq, true, base, &w.own), 256);
+    unsigned char* p = static_cast<unsigned char*>(base);
+    if (prefix_len > 0) {
+        int parts;
+        if (kv->dtype == SA_F32) parts = w.n_split = f32_prefix_splits(ctx, kv, hq, prefix_len);
+        else w.n_split = tc_prefix_splits(ctx, kv, hq, prefix_len, &parts);
+        const size_t rows = (size_t)parts * kv->n_seqs * hq;
+        w.part_o = reinterpret_cast<float*>(p ? p + at : nullptr);
+        at += align_up(rows * kv->d * 4, 256);
+        w.part_ml = reinterpret_cast<float*>(p ? p + at : nullptr);
+        at += align_up(rows * 8, 256);
+    }
+    if (ws) *ws = w;
+    return at;
+}
+
+static int check_tiled(const char* fn, const sa_paged_kv* kv) {
+    SA_CHECK_ARG(kv->d == 64 || kv->d == 128, "%s: d = %d (supported: 64, 128)", fn, kv->d);
+    return SA_OK;
+}
+
+}  // namespace pg
+}  // namespace sa
+
+SA_API int sa_attn_paged_prefill(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_tok_stride, int n_tokens,
+                                 int hq, const int* cu_q, int window, int sinks, float scale, void* out,
+                                 long long o_tok_stride) {
+    using namespace sa;
+    const char* fn = "sa_attn_paged_prefill";
+    clear_error();
+    SA_RC_TRY(pg::check_cache(fn, kv));
+    SA_RC_TRY(pg::check_tiled(fn, kv));
+    SA_RC_TRY(pg::check_heads(fn, kv, hq));
+    SA_RC_TRY(pg::check_scale(fn, scale));
+    SA_CHECK_ARG(window >= 0 && sinks >= 0, "%s: window %d, sinks %d", fn, window, sinks);
+    SA_CHECK_ARG(n_tokens >= 0, "%s: n_tokens %d", fn, n_tokens);
+    if (n_tokens == 0 || kv->n_seqs == 0) return SA_OK;
+    const int e = kv->dtype == SA_F32 ? 4 : 2;
+    SA_CHECK_ARG(cu_q != nullptr, "%s: cu_q is NULL", fn);
+    SA_RC_TRY(pg::check_rows(fn, "q", q, q_tok_stride, (long long)hq * kv->d, e));
+    SA_RC_TRY(pg::check_rows(fn, "out", out, o_tok_stride, (long long)hq * kv->d, e));
+    SA_CHECK_ARG(ctx != nullptr, "%s: ctx is NULL", fn);
+    DeviceGuard guard(ctx->device);
+    if (kv->dtype == SA_F32)
+        return pg::f32_prefill_launch(ctx, kv, static_cast<const float*>(q), q_tok_stride, n_tokens, hq, cu_q, window,
+                                      sinks, scale, static_cast<float*>(out), o_tok_stride);
+    return pg::tc_prefill_launch(ctx, kv, q, q_tok_stride, n_tokens, hq, cu_q, window, sinks, scale, out, o_tok_stride);
+}
+
+static int check_prefix(const char* fn, const sa_paged_kv* kv, int hq, const int* prefix_table, int prefix_len) {
+    using namespace sa;
+    SA_RC_TRY(pg::check_cache(fn, kv));
+    SA_RC_TRY(pg::check_tiled(fn, kv));
+    SA_RC_TRY(pg::check_heads(fn, kv, hq));
+    SA_CHECK_ARG(prefix_len >= 0 && prefix_len <= 0x7ffffe00, "%s: prefix_len %d", fn, prefix_len);
+    SA_CHECK_ARG(prefix_len == 0 || prefix_table, "%s: prefix_table is NULL", fn);
+    return SA_OK;
+}
+
+SA_API int sa_attn_paged_decode_prefix_workspace(sa_ctx* ctx, const sa_paged_kv* kv, int hq, int prefix_len,
+                                                 size_t* bytes) {
+    using namespace sa;
+    const char* fn = "sa_attn_paged_decode_prefix_workspace";
+    clear_error();
+    static const int any = 0;
+    SA_RC_TRY(check_prefix(fn, kv, hq, &any, prefix_len));
+    SA_CHECK_ARG(ctx && bytes, "%s: NULL argument", fn);
+    *bytes = pg::prefix_ws_layout(ctx, kv, hq, prefix_len, nullptr, nullptr);
+    return SA_OK;
+}
+
+SA_API int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const int* prefix_table, int prefix_len,
+                                       const void* q, long long q_stride, int hq, float scale, void* out,
+                                       long long o_stride, void* workspace, size_t workspace_bytes) {
+    using namespace sa;
+    const char* fn = "sa_attn_paged_decode_prefix";
+    clear_error();
+    SA_RC_TRY(check_prefix(fn, kv, hq, prefix_table, prefix_len));
+    SA_RC_TRY(pg::check_scale(fn, scale));
+    if (kv->n_seqs == 0) return SA_OK;
+    const int e = kv->dtype == SA_F32 ? 4 : 2, d = kv->d;
+    SA_RC_TRY(pg::check_rows(fn, "q", q, q_stride, (long long)hq * d, e));
+    SA_RC_TRY(pg::check_rows(fn, "out", out, o_stride, (long long)hq * d, e));
+    SA_CHECK_ARG(ctx != nullptr, "%s: ctx is NULL", fn);
+    DeviceGuard guard(ctx->device);
+    pg::PrefixWs ws;
+    const size_t need = pg::prefix_ws_layout(ctx, kv, hq, prefix_len, workspace, &ws);
+    SA_CHECK_ARG(workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need,
+                 "%s: workspace of %zu bytes (want %zu, 256-byte aligned)", fn, workspace_bytes, need);
+    pg::JoinArgs j;
+    j.c = pg::make_cache(ctx, kv);
+    j.ws = ws.own;
+    j.out = out;
+    j.o_stride = o_stride;
+    j.hq = hq;
+    j.G = hq / kv->hkv;
+    j.n_split = ws.n_split;
+    j.part_o = ws.part_o;
+    j.part_ml = ws.part_ml;
+    j.alt_from = kv->n_seqs;
+    if (prefix_len > 0) {
+        if (kv->dtype == SA_F32) {
+            SA_RC_TRY(pg::f32_prefix_launch(ctx, kv, static_cast<const float*>(q), q_stride, hq, prefix_table,
+                                            prefix_len, scale, ws.n_split, ws.part_o, ws.part_ml));
+        } else {
+            SA_RC_TRY(pg::tc_prefix_launch(ctx, kv, q, q_stride, hq, prefix_table, prefix_len, scale, ws.n_split,
+                                           ws.part_o, ws.part_ml));
+            j.alt_from = pg::tc_prefix_alt_from(kv->n_seqs, j.G);
+        }
+    }
+    SA_RC_TRY(pg::decode_launch(ctx, kv, q, q_stride, hq, 0, 0, scale, nullptr, 0, true, ws.own));
+    const long long rows = (long long)kv->n_seqs * hq, per = pg::JT / (d / 4);
+    const dim3 grid((unsigned)((rows + per - 1) / per));
+    auto k = kv->dtype == SA_F32 ? (d == 64 ? pg::prefix_join_kernel<float, 64> : pg::prefix_join_kernel<float, 128>)
+                                 : (d == 64 ? pg::prefix_join_kernel<__nv_bfloat16, 64>
+                                            : pg::prefix_join_kernel<__nv_bfloat16, 128>);
+    SA_CUDA_TRY(launch_pdl(k, grid, dim3(pg::JT), 0, ctx->stream, j));
+    return SA_OK;
+}

@@ -1,0 +1,560 @@
+// sa_paged_tc.cu -- attention of many query rows over a paged bf16 KV cache on
+// the 5th-generation tensor cores: causal prefill of a ragged batch of prompt
+// chunks with a sliding window and first tokens that stay visible, and the part
+// of a shared-prefix decode that all sequences have in common.
+//
+//   out[i] = sum_j w_ij v_j / sum_j w_ij,  w_ij = 2^(scale log2(e) q_i . k_j - m_i)
+// over the rows j that query i sees; m_i is a running maximum.
+//
+// Rows of a tile: the G = hq / hkv query heads of one KV head for 128 / G
+// consecutive tokens, so that every K/V tile serves all heads that read it and
+// a window's edges cost the tiles of few tokens.  A CTA holds two such slots of
+// 128 rows over the same K/V tiles (neighbouring tokens); the tensor core works
+// for one while the other's softmax runs.
+//
+// The prefix of a shared-prefix decode has no mask: query rows are (sequence,
+// head) pairs, the keys are split over CTAs, each leaving (m, l, O) for a join.
+// With at most 128 rows per KV head the two slots hold the same rows and take
+// alternate key tiles, which keeps the overlap that two slots give.
+//
+// Warp roles, TMEM and the softmax are those of the causal prefill kernel
+// (sa_prefill.cu): warp 0 issues TMA loads, one lane of warp 1 the MMAs, warps
+// 4-7 and 8-11 are the softmax warpgroups of the slots (a thread per row).
+// What pages change:
+//  * a tile of 128 keys arrives as one box per page and 64-column half, issued
+//    by the producer's lanes in parallel, with the block-table entries of the
+//    next tile fetched while the ring is full;
+//  * a page that none of the CTA's queries sees is not looked up: its box is
+//    asked for at a page past the pool, which TMA fills with zeros;
+//  * rows behind the sequence's last one share a page with it and may hold
+//    anything: K's are masked, V's are overwritten with zeros in shared memory
+//    by the softmax threads before the tile's P is handed over.
+#include <algorithm>
+#include <cmath>
+
+#include "sa_fa.cuh"
+#include "sa_paged.cuh"
+#include "sa_paged_decode.h"
+#include "sa_paged_tc.h"
+
+namespace sa {
+namespace pg {
+
+using pf::BM;
+using pf::BN;
+using pf::col_o;
+using pf::col_p;
+using pf::col_s;
+using pf::wait_ab;
+
+constexpr int TC_THREADS = 384;
+constexpr int TC_REG_CTRL = 72, TC_REG_SOFTMAX = 216;      // 128 * 72 + 256 * 216 = 384 * 168
+constexpr int BOX = 128 * 128;                             // 128 rows of 64 bf16
+
+template <int D>
+struct Lay {
+    static constexpr int HALVES = D / 64;
+    static constexpr int TILE = HALVES * BOX;
+    static constexpr int ST = D == 64 ? 4 : 2;             // ring depth, K and V each
+    static constexpr int Q = 0, K = 2 * TILE, V = K + ST * TILE, BAR = V + ST * TILE;
+    static constexpr int SMEM = BAR + 512 + 1024;
+};
+
+struct TcArgs {
+    Cache c;
+    const int* cu_q;           // prefill
+    int n_tok;                 // query rows of the q tensor: tokens, or sequences
+    int G, tpt;                // heads per KV head; tokens per tile, 128 / G
+    int window, sinks;
+    float sl2;                 // scale * log2(e)
+    void* out;                 // prefill: bf16
+    long long o_tok;
+    // shared prefix
+    int prefix_len, n_split, units;
+    const int* prefix_table;
+    float* part_o;             // [parts][n_tok * hq][D], unnormalised
+    float* part_ml;            // [parts][n_tok * hq][2]
+    int hq;
+};
+
+template <int ST>
+struct TcBars {
+    uint64_t q_full;
+    uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST];
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t drain;
+    uint32_t tmem_base;
+    int abort;
+};
+
+// What this CTA computes.
+struct Unit {
+    int b, kvh;
+    int tok0[2], ntok[2];      // rows of the q tensor
+    int p0[2];                 // position of the slot's first query (prefill)
+    int len;                   // rows of the sequence / the prefix
+    UnitTiles u;
+    int j0;                    // first tile (prefix: of the split)
+    bool alt;                  // both slots hold the same rows and take alternate tiles
+};
+
+// Prefill: CTA u takes unit total - 1 - u of the batch's (the last tokens of a
+// sequence see the most rows: they start first).
+__device__ bool find_prefill_unit(const TcArgs& a, Unit* s, SeqUnit* su, int* scan) {
+    if (!find_seq_unit<TC_THREADS>(a.c, a.cu_q, a.n_tok, 2 * a.tpt, blockIdx.x / a.c.hkv, su, scan)) return false;
+    if (threadIdx.x == 0) {
+        s->b = su->b;
+        s->kvh = blockIdx.x % a.c.hkv;
+        s->len = seq_len(a.c, su->b);
+        int last[2];
+        for (int x = 0; x < 2; ++x) {
+            const int t = (2 * su->unit + x) * a.tpt;
+            s->tok0[x] = su->first + t;
+            s->ntok[x] = max(0, min(a.tpt, su->tokens - t));
+            s->p0[x] = s->len - su->tokens + t;
+            last[x] = s->ntok[x] ? max(-1, s->p0[x] + s->ntok[x] - 1) : -1;
+        }
+        s->u = make_unit(s->p0[0], last[0], last[1], a.window, a.sinks, BN);
+        s->j0 = 0;
+        s->alt = false;
+    }
+    __syncthreads();
+    return true;
+}
+// Prefix: CTA = (split, KV head, pair of row tiles), the pair fastest, so that
+// CTAs that read the same keys run side by side.
+__device__ void find_prefix_unit(const TcArgs& a, Unit* s) {
+    if (threadIdx.x == 0) {
+        const int unit = blockIdx.x % a.units, r = blockIdx.x / a.units;
+        const int split = r / a.c.hkv;
+        const int tiles = (int)(((long long)a.prefix_len + BN - 1) / BN);
+        s->b = 0;
+        s->kvh = r % a.c.hkv;
+        s->len = a.prefix_len;
+        for (int x = 0; x < 2; ++x) {
+            s->tok0[x] = (2 * unit + x) * a.tpt;
+            s->ntok[x] = max(0, min(a.tpt, a.n_tok - s->tok0[x]));
+            s->p0[x] = a.prefix_len;
+        }
+        s->j0 = (int)share_first(split, tiles, a.n_split);
+        const int n = (int)share_first(split + 1, tiles, a.n_split) - s->j0;
+        s->alt = s->ntok[1] == 0;
+        if (s->alt) {
+            s->tok0[1] = s->tok0[0];
+            s->ntok[1] = s->ntok[0];
+        }
+        s->u = make_unit(0, a.prefix_len - 1, a.prefix_len - 1, 0, 0, BN);
+        s->u.t.n = n;
+        s->u.n[0] = s->alt ? (n + 1) / 2 : n;
+        s->u.n[1] = s->alt ? n / 2 : n;
+    }
+    __syncthreads();
+}
+
+template <int D, bool PREFIX>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                const __grid_constant__ CUtensorMap tv, const __grid_constant__ TcArgs a) {
+    using L = Lay<D>;
+    constexpr int ST = L::ST;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ Unit s_unit;
+    __shared__ SeqUnit s_seq;
+    __shared__ int s_scan[TC_THREADS / 32];
+    const uint32_t raw = smem_u32(smem_raw);
+    unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+    TcBars<ST>* B = reinterpret_cast<TcBars<ST>*>(sm + L::BAR);
+    volatile int* abort = &B->abort;
+    int* status = a.c.status;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (PREFIX) pdl_trigger();
+
+    if constexpr (PREFIX) find_prefix_unit(a, &s_unit);
+    else if (!find_prefill_unit(a, &s_unit, &s_seq, s_scan)) return;      // the same for every thread
+    const Tiles t = s_unit.u.t;
+    const int n_kv = t.n, kvh = s_unit.kvh;
+    const int n0 = s_unit.u.n[0], n1 = s_unit.u.n[1];
+    const bool alt = s_unit.alt;
+
+    if (tid == 0) {
+        mbar_init(&B->q_full, 1);
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(&B->k_full[s], 1);
+            mbar_init(&B->k_empty[s], 1);
+            mbar_init(&B->v_full[s], 1);
+            mbar_init(&B->v_empty[s], 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(&B->s_full[x], 1);
+            mbar_init(&B->p_full[x], 4);
+            mbar_init(&B->o_full[x], 1);
+        }
+        mbar_init(&B->drain, 1);
+        B->abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) tc::tmem_alloc(&B->tmem_base, 512);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tbase = B->tmem_base;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_REG_CTRL));
+        if (warp == 0 && n_kv > 0) {
+            // ---------------------------------------------- TMA producer
+            if (lane == 0) {
+                tc::prefetch_tmap(&tq);
+                tc::prefetch_tmap(&tk);
+                tc::prefetch_tmap(&tv);
+                const int slots = (alt || s_unit.ntok[1] == 0) ? 1 : 2;
+                mbar_arrive_expect_tx(&B->q_full, (uint32_t)(slots * L::HALVES * a.tpt * a.G * 128));
+                for (int x = 0; x < slots; ++x)
+                    for (int f = 0; f < L::HALVES; ++f)
+                        tc::tma_load_3d(sm + L::Q + x * L::TILE + f * BOX, &tq, f * 64, kvh * a.G, s_unit.tok0[x],
+                                        &B->q_full);
+            }
+            const int pl = a.c.page_log2, page = 1 << pl, copies = BN >> pl;
+            const int* row = PREFIX ? a.prefix_table : a.c.table + (long long)s_unit.b * a.c.table_stride;
+            const int j0 = s_unit.j0;
+            auto wanted = [&](int j) { return lane < copies && t.any(t.row0(j0 + j, BN) + lane * page, page); };
+            auto entry = [&](int j) { return wanted(j) ? row[(t.row0(j0 + j, BN) + lane * page) >> pl] : -1; };
+            int next = entry(0);
+            int k_issued = 0, v_issued = 0;
+            for (int j = 0; j < n_kv; ++j) {
+                const int s = j % ST;
+                int pg_id = a.c.n_pages;                         // past the pool: zeros
+                if (wanted(j)) {
+                    pg_id = checked_page(a.c, next);
+                    if (pg_id < 0) pg_id = a.c.n_pages;
+                }
+                if (j + 1 < n_kv) next = entry(j + 1);
+                const uint32_t par = ((j / ST) & 1) ^ 1;
+                bool ok = j < ST || wait_ab(&B->k_empty[s], par, abort, status);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                if (lane == 0) mbar_arrive_expect_tx(&B->k_full[s], L::TILE);
+                __syncwarp();
+                if (lane < copies)
+                    for (int f = 0; f < L::HALVES; ++f)
+                        tc::tma_load_3d(sm + L::K + s * L::TILE + f * BOX + lane * page * 128, &tk, f * 64, kvh << pl,
+                                        pg_id, &B->k_full[s]);
+                k_issued = j + 1;
+                ok = j < ST || wait_ab(&B->v_empty[s], par, abort, status);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                if (lane == 0) mbar_arrive_expect_tx(&B->v_full[s], L::TILE);
+                __syncwarp();
+                if (lane < copies)
+                    for (int f = 0; f < L::HALVES; ++f)
+                        tc::tma_load_3d(sm + L::V + s * L::TILE + f * BOX + lane * page * 128, &tv, f * 64, kvh << pl,
+                                        pg_id, &B->v_full[s]);
+                v_issued = j + 1;
+            }
+            if (*abort) {                                       // let the loads in flight land
+                mbar_wait(&B->q_full, 0, nullptr);
+                for (int j = max(0, k_issued - ST); j < k_issued; ++j)
+                    mbar_wait(&B->k_full[j % ST], (j / ST) & 1, nullptr);
+                for (int j = max(0, v_issued - ST); j < v_issued; ++j)
+                    mbar_wait(&B->v_full[j % ST], (j / ST) & 1, nullptr);
+            }
+        } else if (warp == 1 && lane == 0 && n_kv > 0) {
+            // ---------------------------------------------- MMA issuer
+            constexpr uint32_t idS = tc::idesc_bf16_f32(BM, BN, false, false);
+            constexpr uint32_t idO = tc::idesc_bf16_f32(BM, D, false, true);
+            const uint32_t sQ = smem_u32(sm + L::Q), sK = smem_u32(sm + L::K), sV = smem_u32(sm + L::V);
+            auto issue_S = [&](int x, int j) {
+                const uint32_t q = sQ + (alt ? 0 : x) * L::TILE, k = sK + (j % ST) * L::TILE;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t off = (kk >> 2) * BOX + (kk & 3) * 32;
+                    tc::mma_bf16(tbase + col_s(x), tc::sdesc_sw128(q + off, 16, 1024),
+                                 tc::sdesc_sw128(k + off, 16, 1024), idS, kk > 0);
+                }
+            };
+            auto issue_PV = [&](int x, int j, bool first) {
+                const uint32_t v = sV + (j % ST) * L::TILE;
+#pragma unroll
+                for (int kk = 0; kk < BN / 16; ++kk)
+                    tc::mma_bf16_ts(tbase + col_o(x), tbase + col_p(x) + kk * 8,
+                                    tc::sdesc_sw128(v + kk * 2048, BOX, 1024), idO, (!first || kk > 0) ? 1u : 0u);
+            };
+            auto k_ready = [&](int j) { return wait_ab(&B->k_full[j % ST], (j / ST) & 1, abort, status); };
+            auto v_ready = [&](int j) { return wait_ab(&B->v_full[j % ST], (j / ST) & 1, abort, status); };
+            bool ok = wait_ab(&B->q_full, 0, abort, status);
+            if (alt) {
+                for (int x = 0; ok && x < 2 && x < n_kv; ++x) {
+                    if (!(ok = k_ready(x))) break;
+                    tc::fence_after_sync();
+                    issue_S(x, x);
+                    tc::mma_commit(&B->s_full[x]);
+                    tc::mma_commit(&B->k_empty[x % ST]);
+                }
+                for (int j = 0; ok && j < n_kv; ++j) {
+                    const int x = j & 1, c = j >> 1;
+                    if (!(ok = v_ready(j) && wait_ab(&B->p_full[x], c & 1, abort, status))) break;
+                    tc::fence_after_sync();
+                    issue_PV(x, j, c == 0);
+                    tc::mma_commit(&B->v_empty[j % ST]);
+                    if (j + 2 >= n_kv) {
+                        tc::mma_commit(&B->o_full[x]);
+                        continue;
+                    }
+                    if (!(ok = k_ready(j + 2))) break;
+                    tc::fence_after_sync();
+                    issue_S(x, j + 2);
+                    tc::mma_commit(&B->s_full[x]);
+                    tc::mma_commit(&B->k_empty[(j + 2) % ST]);
+                }
+            } else {
+                ok = ok && k_ready(0);
+                tc::fence_after_sync();
+                if (ok) {
+                    for (int x = 0; x < 2; ++x)
+                        if (0 < (x ? n1 : n0)) {
+                            issue_S(x, 0);
+                            tc::mma_commit(&B->s_full[x]);
+                        }
+                    tc::mma_commit(&B->k_empty[0]);
+                }
+                for (int j = 0; ok && j < n_kv; ++j) {
+                    if (!(ok = v_ready(j))) break;
+                    bool k_next = false;
+                    for (int x = 0; ok && x < 2; ++x) {
+                        const int nx = x ? n1 : n0;
+                        if (j >= nx) continue;
+                        if (!(ok = wait_ab(&B->p_full[x], j & 1, abort, status))) break;
+                        tc::fence_after_sync();
+                        issue_PV(x, j, j == 0);
+                        if (j + 1 == nx) {
+                            tc::mma_commit(&B->o_full[x]);
+                            continue;
+                        }
+                        if (!k_next) {
+                            if (!(ok = k_ready(j + 1))) break;
+                            tc::fence_after_sync();
+                            k_next = true;
+                        }
+                        issue_S(x, j + 1);
+                        tc::mma_commit(&B->s_full[x]);
+                    }
+                    if (!ok) break;
+                    tc::mma_commit(&B->v_empty[j % ST]);
+                    if (k_next) tc::mma_commit(&B->k_empty[(j + 1) % ST]);
+                }
+            }
+            tc::mma_commit(&B->drain);                          // issued MMAs complete before TMEM is released
+            mbar_wait(&B->drain, 0, nullptr);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_REG_SOFTMAX));
+        // ---------------------------------------------- softmax warpgroups
+        const int x = (warp - 4) >> 2;
+        const int ntok = s_unit.ntok[x];
+        if (ntok > 0) {
+            const int quad = warp & 3, row = quad * 32 + lane;
+            const uint32_t lane_addr = tbase + ((uint32_t)(quad * 32) << 16);
+            const int tok = row / a.G, g = row - tok * a.G;
+            const int nx = x ? n1 : n0, p0 = s_unit.p0[x];
+            const int len = s_unit.len;
+            // what this row sees: [lo, lo + span) and [0, first)
+            const int limit = PREFIX ? len - 1 : p0 + tok;
+            const int lo = PREFIX ? 0 : window_lo(limit, a.window);
+            const unsigned span = limit < 0 ? 0u : (unsigned)(limit - lo + 1);
+            const int first = PREFIX ? 0 : min(a.sinks, limit + 1);
+            // what every row of the slot sees
+            const int all_hi = PREFIX ? len - 1 : p0;
+            const int all_lo = PREFIX ? 0 : window_lo(p0 + ntok - 1, a.window);
+            const float sl2 = a.sl2;
+            float m = -INFINITY, l = 0.f;
+            bool ok = true;
+            for (int c = 0; c < nx; ++c) {
+                const int j = alt ? 2 * c + x : c;
+                if (!(ok = wait_ab(&B->s_full[x], c & 1, abort, status))) break;
+                tc::fence_after_sync();
+                uint32_t u32[BN];
+#pragma unroll
+                for (int cb = 0; cb < BN / 32; ++cb) tc::tmem_ld32p(lane_addr + col_s(x) + cb * 32, u32 + cb * 32);
+                tc::tmem_wait_ld();
+                float* sc = reinterpret_cast<float*>(u32);
+                const int k0 = t.row0(s_unit.j0 + j, BN);
+                if (k0 + BN - 1 > all_hi || !(k0 >= all_lo || k0 + BN <= a.sinks)) {
+                    const int rel = k0 - lo;
+#pragma unroll
+                    for (int i = 0; i < BN; ++i)
+                        if ((unsigned)(rel + i) >= span && k0 + i >= first) sc[i] = -INFINITY;
+                }
+                const uint32_t p_addr = lane_addr + col_p(x);
+                float alpha = 1.f, sum;
+                if (c == 0) {
+                    m = pf::row_max(sc) * sl2;
+                    sum = pf::emit_p<0, false>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, nullptr);
+                } else {
+                    float mxr;
+                    sum = pf::emit_p<0, true>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, &mxr);
+                    const float mxs = mxr * sl2;
+                    const bool need = mxs > m + pf::RESCALE_THRESHOLD;
+                    if (__any_sync(0xffffffffu, need)) {
+                        if (need) {
+                            alpha = ex2(m - mxs);
+                            m = mxs;
+                        }
+#pragma unroll 1
+                        for (int cb = 0; cb < D / 32; ++cb) {
+                            uint32_t o[32];
+                            tc::tmem_ld32(lane_addr + col_o(x) + cb * 32, o);
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tc::tmem_st32(lane_addr + col_o(x) + cb * 32, o);
+                        }
+                        tc::tmem_wait_st();
+                        sum = pf::emit_p<0, false>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, nullptr);
+                    }
+                }
+                l = l * alpha + sum;
+                // rows behind the last one enter P.V as zeros; the first slot that
+                // uses the tile clears them (the other's P.V is issued later)
+                if (k0 + BN > len && (alt || x == 0 || j >= n0)) {
+                    const int s = j % ST, r0 = max(0, len - k0), n = (BN - r0) * 8 * L::HALVES;
+                    if (!(ok = wait_ab(&B->v_full[s], (j / ST) & 1, abort, status))) break;
+                    for (int i = row; i < n; i += BM) {
+                        const int f = i / ((BN - r0) * 8), e = i - f * (BN - r0) * 8;
+                        *reinterpret_cast<uint4*>(sm + L::V + s * L::TILE + f * BOX + r0 * 128 + e * 16) =
+                            make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                }
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B->p_full[x]);
+            }
+            const bool mine = tok < ntok && row < a.tpt * a.G;
+            if (ok && (nx == 0 || wait_ab(&B->o_full[x], 0, abort, status))) {
+                tc::fence_after_sync();
+                const long long qrow = s_unit.tok0[x] + tok;
+                const int h = kvh * a.G + g;
+                if constexpr (PREFIX) {
+                    const int split = (int)(blockIdx.x / a.units) / a.c.hkv;
+                    const long long part = alt ? 2 * split + x : split;
+                    const long long at = (part * a.n_tok + qrow) * a.hq + h;
+                    if (mine) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+#pragma unroll 1
+                    for (int cb = 0; cb < D / 32; ++cb) {
+                        uint32_t o[32];
+                        if (nx > 0) {
+                            tc::tmem_ld32(lane_addr + col_o(x) + cb * 32, o);
+                            tc::tmem_wait_ld();
+                        }
+                        if (!mine || nx == 0) continue;          // an empty part is known by its m
+                        float* dst = a.part_o + at * D + cb * 32;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4*>(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
+                } else {
+                    const float inv = l > 0.f ? 1.f / l : 0.f;
+                    __nv_bfloat16* dst0 = static_cast<__nv_bfloat16*>(a.out) + qrow * a.o_tok + (long long)h * D;
+#pragma unroll 1
+                    for (int cb = 0; cb < D / 32; ++cb) {
+                        uint32_t o[32];
+                        if (nx > 0) {
+                            tc::tmem_ld32(lane_addr + col_o(x) + cb * 32, o);
+                            tc::tmem_wait_ld();
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = 0u;
+                        }
+                        if (!mine) continue;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                w[e] = pf::pack_bf16(__uint_as_float(o[i + 2 * e]) * inv,
+                                                     __uint_as_float(o[i + 2 * e + 1]) * inv);
+                            *reinterpret_cast<uint4*>(dst0 + cb * 32 + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tbase, 512);
+    }
+}
+
+template <int D, bool PREFIX>
+static int tc_launch_d(cudaStream_t st, int grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+                       const TcArgs& a) {
+    auto k = paged_tc_kernel<D, PREFIX>;
+    SA_RC_TRY(set_smem_attr_once((const void*)k, Lay<D>::SMEM));
+    k<<<grid, TC_THREADS, Lay<D>::SMEM, st>>>(mq, mk, mv, a);
+    SA_CUDA_TRY(cudaGetLastError());
+    return SA_OK;
+}
+
+static int tc_maps(const sa_paged_kv* kv, const void* q, long long q_tok, int n_tok, int hq, TcArgs* a, CUtensorMap* mq,
+                   CUtensorMap* mk, CUtensorMap* mv) {
+    a->G = hq / kv->hkv;
+    a->tpt = BM / a->G;
+    a->hq = hq;
+    a->n_tok = n_tok;
+    SA_RC_TRY(make_query_tmap(mq, q, kv->d, hq, n_tok, q_tok, a->G, a->tpt));
+    SA_RC_TRY(make_page_tmap(mk, kv->k_pages, kv, kv->page_size));
+    return make_page_tmap(mv, kv->v_pages, kv, kv->page_size);
+}
+
+int tc_prefill_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_tok, int n_tok, int hq,
+                      const int* cu_q, int window, int sinks, float scale, void* out, long long o_tok) {
+    TcArgs a = {};
+    CUtensorMap mq, mk, mv;
+    SA_RC_TRY(tc_maps(kv, q, q_tok, n_tok, hq, &a, &mq, &mk, &mv));
+    a.c = make_cache(ctx, kv);
+    a.cu_q = cu_q;
+    a.window = window;
+    a.sinks = sinks;
+    a.sl2 = scale * pf::LOG2E;
+    a.out = out;
+    a.o_tok = o_tok;
+    // every sequence's last unit may be partly filled
+    const long long units = (long long)n_tok / (2 * a.tpt) + std::min(kv->n_seqs, n_tok);
+    const long long grid = units * kv->hkv;
+    SA_CHECK_ARG(grid < (1LL << 31), "prefill: %lld CTAs", grid);
+    return kv->d == 64 ? tc_launch_d<64, false>(ctx->stream, (int)grid, mq, mk, mv, a)
+                       : tc_launch_d<128, false>(ctx->stream, (int)grid, mq, mk, mv, a);
+}
+
+// One CTA per SM: as many key splits as fill the GPU, no split without a tile.
+int tc_prefix_splits(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, int prefix_len, int* parts) {
+    const int tpt = BM / (hq / kv->hkv), units = ((kv->n_seqs + tpt - 1) / tpt + 1) / 2;
+    const int tiles = (int)(((long long)prefix_len + BN - 1) / BN);
+    const int n = std::max(1, std::min(tiles, ctx->num_sms / std::max(1, units * kv->hkv)));
+    *parts = 2 * n;
+    return n;
+}
+
+int tc_prefix_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_tok, int hq, const int* prefix_table,
+                     int prefix_len, float scale, int n_split, float* part_o, float* part_ml) {
+    TcArgs a = {};
+    CUtensorMap mq, mk, mv;
+    SA_RC_TRY(tc_maps(kv, q, q_tok, kv->n_seqs, hq, &a, &mq, &mk, &mv));
+    a.c = make_cache(ctx, kv);
+    a.sl2 = scale * pf::LOG2E;
+    a.prefix_table = prefix_table;
+    a.prefix_len = prefix_len;
+    a.n_split = n_split;
+    a.units = ((kv->n_seqs + a.tpt - 1) / a.tpt + 1) / 2;
+    a.part_o = part_o;
+    a.part_ml = part_ml;
+    const long long grid = (long long)a.units * kv->hkv * n_split;
+    SA_CHECK_ARG(grid < (1LL << 31), "prefix: %lld CTAs", grid);
+    return kv->d == 64 ? tc_launch_d<64, true>(ctx->stream, (int)grid, mq, mk, mv, a)
+                       : tc_launch_d<128, true>(ctx->stream, (int)grid, mq, mk, mv, a);
+}
+
+}  // namespace pg
+}  // namespace sa

@@ -196,3 +196,54 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, kv_lens, scale: float, w
     check(L.sa_attn_paged_decode(ctx.h, C.byref(kv), q.data_ptr(), qs, q.shape[1], window, sinks, scale, out.data_ptr(),
                                  os, ws.data_ptr(), n))
     return out
+
+
+def attn_paged_prefill(q, k_pages, v_pages, block_table, kv_lens, cu_q, scale: float, window: int = 0, sinks: int = 0,
+                       ctx: Context | None = None, out=None):
+    """A ragged batch of prompt chunks over the sequences' pages (sa_attn_paged_prefill).
+
+    q [n_tokens, hq, d] in the pages' dtype, d 64 or 128: tokens
+    cu_q[b] .. cu_q[b + 1] - 1 are the last ones of sequence b, whose keys and
+    values have been appended.  Causal, with ``window`` and ``sinks`` as in
+    attn_paged_decode.  Returns [n_tokens, hq, d]; rows behind the last
+    sequence are left as they were.
+    """
+    kv = _cache(k_pages, v_pages, block_table, kv_lens)
+    dev = k_pages.device
+    qs = _rows(q, "q", None, kv.d, dev, k_pages.dtype)
+    if not _index(cu_q, "cu_q", (kv.n_seqs + 1,), dev).is_contiguous():
+        raise ValueError("cu_q: must be contiguous")
+    out = _out(out, q, dev)
+    os = _rows(out, "out", q.shape[1], kv.d, dev, q.dtype)
+    ctx = _bind(ctx, dev)
+    check(lib().sa_attn_paged_prefill(ctx.h, C.byref(kv), q.data_ptr(), qs, q.shape[0], q.shape[1], cu_q.data_ptr(),
+                                      window, sinks, scale, out.data_ptr(), os))
+    return out
+
+
+def attn_paged_decode_prefix(q, k_pages, v_pages, prefix_table, prefix_len: int, block_table, kv_lens, scale: float,
+                             ctx: Context | None = None, out=None):
+    """One query token per sequence behind a prefix that all share (sa_attn_paged_decode_prefix).
+
+    prefix_table [>= ceil(prefix_len / page_size)] int32 lists the prefix's
+    pages; block_table and kv_lens are those of each sequence's own rows (a
+    length may be 0).  q [n_seqs, hq, d] sees all of both.  d 64 or 128.
+    Returns [n_seqs, hq, d].
+    """
+    kv = _cache(k_pages, v_pages, block_table, kv_lens)
+    dev = k_pages.device
+    qs = _rows(q, "q", None, kv.d, dev, k_pages.dtype)
+    if q.shape[0] != kv.n_seqs:
+        raise ValueError(f"q has {q.shape[0]} tokens, the block table {kv.n_seqs} sequences")
+    if prefix_table.dim() != 1 or prefix_table.shape[0] * kv.page_size < prefix_len:
+        raise ValueError(f"prefix_table: shape {tuple(prefix_table.shape)} for {prefix_len} rows")
+    if not _index(prefix_table, "prefix_table", prefix_table.shape, dev).is_contiguous():
+        raise ValueError("prefix_table: must be contiguous")
+    out = _out(out, q, dev)
+    os = _rows(out, "out", q.shape[1], kv.d, dev, q.dtype)
+    ctx = _bind(ctx, dev)
+    L = lib()
+    ws, n = _workspace(L.sa_attn_paged_decode_prefix_workspace, dev, ctx.h, C.byref(kv), q.shape[1], prefix_len)
+    check(L.sa_attn_paged_decode_prefix(ctx.h, C.byref(kv), prefix_table.data_ptr(), prefix_len, q.data_ptr(), qs,
+                                        q.shape[1], scale, out.data_ptr(), os, ws.data_ptr(), n))
+    return out

@@ -30,6 +30,16 @@ def _append(kv, xd=SA_BF16, q=P, qs=4 * 128, k=P, ks=256, v=P, vs=256, n=5, hq=4
                                  cos, sin, n_pos, rot, inter, qo, qos)
 
 
+def _prefill(kv, q=P, qs=512, n=5, hq=4, cu=P, window=0, sinks=0, scale=1.0, out=P, os=512):
+    return lib().sa_attn_paged_prefill(None, C.byref(kv) if kv is not None else None, q, qs, n, hq, cu, window, sinks,
+                                       scale, out, os)
+
+
+def _prefix(kv, table=P, n=100, q=P, qs=512, hq=4, scale=1.0, out=P, os=512, ws=P, nb=1 << 30):
+    return lib().sa_attn_paged_decode_prefix(None, C.byref(kv) if kv is not None else None, table, n, q, qs, hq, scale,
+                                             out, os, ws, nb)
+
+
 def _refused(rc, text):
     msg = lib().sa_last_error().decode()
     assert rc == -1 and text in msg, (rc, msg)
@@ -49,12 +59,42 @@ BAD_CACHE = [(dict(dtype=7), "dtype 7"), (dict(k_pages=None), "null k_pages"), (
 def test_bad_caches(over, text):
     _refused(_decode(_kv(**over)), text)
     _refused(_append(_kv(**over)), text)
+    _refused(_prefill(_kv(**over)), text)
+    _refused(_prefix(_kv(**over)), text)
+
+
+@pytest.mark.parametrize("over,text", [
+    (dict(hq=3), "hq = 3"), (dict(hq=40, qs=5120, os=5120), "hq = 40"), (dict(window=-5), "window -5"),
+    (dict(sinks=-5), "sinks -5"), (dict(scale=-0.5), "scale"), (dict(n=-1), "n_tokens -1"), (dict(cu=None), "cu_q is NULL"),
+    (dict(q=P + 2), "q is NULL or not"), (dict(qs=504), "q token stride"), (dict(out=None), "out is NULL"),
+    (dict(os=511), "out token stride")])
+def test_bad_prefill_arguments(over, text):
+    _refused(_prefill(_kv(), **over), text)
+
+
+@pytest.mark.parametrize("over,text", [
+    (dict(hq=3), "hq = 3"), (dict(n=-1), "prefix_len -1"), (dict(n=2 ** 31 - 1), "prefix_len"),
+    (dict(table=None), "prefix_table is NULL"), (dict(scale=0.0), "scale"), (dict(q=None), "q is NULL"),
+    (dict(out=P + 8), "out is NULL or not"), (dict(os=300), "out token stride")])
+def test_bad_prefix_arguments(over, text):
+    _refused(_prefix(_kv(), **over), text)
+
+
+def test_tiled_attention_takes_heads_of_64_and_128():
+    wide = _kv(d=256, page_stride=2 * 16 * 256)
+    _refused(_prefill(wide, qs=1024, os=1024), "d = 256")
+    _refused(_prefix(wide, qs=1024, os=1024), "d = 256")
 
 
 def test_null_description_and_context():
     _refused(_decode(None), "kv is NULL")
     _refused(_append(None), "kv is NULL")
+    _refused(_prefill(None), "kv is NULL")
+    _refused(_prefix(None), "kv is NULL")
     _refused(_decode(_kv()), "ctx is NULL")
+    _refused(_prefill(_kv()), "ctx is NULL")
+    _refused(_prefix(_kv()), "ctx is NULL")
+    _refused(_prefix(_kv(), table=None, n=0), "ctx is NULL")
     _refused(_append(_kv()), "ctx is NULL")
 
 
@@ -88,6 +128,8 @@ def test_bad_append_arguments(over, text):
 def test_nothing_to_do_is_no_error():
     assert _append(_kv(), n=0, k=None, v=None) == 0
     assert _append(_kv(n_seqs=0, block_table=None, kv_lens=None, max_pages=0)) == 0
+    assert _prefill(_kv(), n=0, q=None, out=None, cu=None) == 0
+    assert _prefix(_kv(n_seqs=0, block_table=None, kv_lens=None, max_pages=0), q=None, out=None) == 0
     assert _decode(_kv(n_seqs=0, block_table=None, kv_lens=None, max_pages=0), q=None, out=None) == 0
 
 

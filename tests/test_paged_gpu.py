@@ -244,3 +244,171 @@ def test_decode_reports_bad_pages_and_lengths():
         good = sa.attn_paged_decode(q, pool.kp, pool.vp, pool.table, pool.kv_lens, 1.0, ctx=ctx)
         ctx.synchronize()
         assert torch.isfinite(good).all()
+
+
+# ---------------------------------------------------------------- prefill
+
+def _prefill(pool, new, hq, window=0, sinks=0, tail=0, ctx=None, scale=None, q_pad=0, spread=1.0):
+    sa = _sa()
+    d, n = pool.d, sum(new)
+    scale = scale or 1.0 / math.sqrt(d)
+    cu = torch.tensor([0] + list(new)).cumsum(0)
+    q = pool.q(n + tail, hq, spread)
+    qd = torch.empty(n + tail, hq + q_pad, d, dtype=pool.dt, device="cuda")
+    qd[:, :hq] = q.cuda()
+    out = torch.full((n + tail, hq + q_pad, d), 5.0, dtype=pool.dt, device="cuda")
+    got = sa.attn_paged_prefill(qd[:, :hq], pool.kp, pool.vp, pool.table, pool.kv_lens, cu.int().cuda(), scale, window=window,
+                                sinks=sinks, ctx=ctx, out=out[:, :hq])
+    ref = torch.cat([attend(q[cu[b]:cu[b + 1]], pool.k[b], pool.v[b], list(range(m - new[b], m)), scale, window, sinks)
+                     for b, m in enumerate(pool.lens)])
+    torch.cuda.synchronize()
+    assert (out[n:] == 5.0).all() and (out[:, hq:] == 5.0).all()
+    return got[:n], ref
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 16), (128, 32), (64, 64), (128, 128)])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 2), (3, 1), (8, 1), (16, 1)])
+def test_prefill_ragged(dtype, d, page, hq, hkv):
+    new = [1, 0, 130, 64, 5, 300]
+    past = [0, 17, 0, 64, 250, 129]
+    pool = Pool([a + b for a, b in zip(past, new)], hkv, d, page, dtype, seed=d + page + hq)
+    out, ref = _prefill(pool, new, hq, tail=3)
+    _close(out, ref, dtype, _v_max(pool))
+
+
+@pytest.mark.parametrize("dtype,d,page,hq,hkv", [("bf16", 128, 16, 4, 2), ("bf16", 64, 32, 8, 1), ("bf16", 128, 128, 2, 2),
+                                                 ("f32", 128, 16, 4, 2), ("f32", 64, 64, 5, 1)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (100, 0), (129, 70), (64, 130), (128, 16), (300, 140),
+                                          (5000, 4)])
+def test_prefill_window(dtype, d, page, hq, hkv, window, sinks):
+    new, past = [200, 3, 77, 1], [500, 0, 13, 300]
+    pool = Pool([a + b for a, b in zip(past, new)], hkv, d, page, dtype, seed=window + sinks)
+    for b, n in enumerate(pool.lens):                      # pages that none of the queries sees have been given back
+        pool.forget(b, lambda r, n=n, m=new[b]: any(sees(p, r, window, sinks) for p in range(n - m, n)))
+    with _sa().Context(0) as ctx:
+        out, ref = _prefill(pool, new, hq, window, sinks, ctx=ctx)
+        ctx.synchronize()
+    _close(out, ref, dtype, _v_max(pool), (window, sinks))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prefill_lengths_around_tiles(dtype):
+    """Lengths and chunk sizes around 64, 128 and the slots' sizes, many sequences in one call."""
+    new, past = [], []
+    for n in (1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257):
+        for p in (0, 1, 127, 128):
+            new.append(n)
+            past.append(p)
+    pool = Pool([a + b for a, b in zip(past, new)], 1, 64, 16, dtype, seed=1)
+    out, ref = _prefill(pool, new, 4, window=90, sinks=2)
+    _close(out, ref, dtype, _v_max(pool))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prefill_scores_of_all_sizes(dtype):
+    pool = Pool([700, 64], 1, 128, 16, dtype, seed=12)
+    out, ref = _prefill(pool, [300, 64], 2, scale=1.0 if dtype == "bf16" else 0.5, spread=2.0, q_pad=1)
+    # as test_decode_scores_of_all_sizes
+    off = (out.double().cpu() - ref).abs()
+    assert (off <= (tolerance(dtype, ref, _v_max(pool)) if dtype == "bf16" else 0) + 1.5e-3 * _v_max(pool)).all()
+
+
+def test_prefill_more_sequences_than_threads():
+    new = [(5 * i) % 4 for i in range(900)]
+    pool = Pool([n + i % 3 for i, n in enumerate(new)], 1, 64, 16, "bf16", seed=13)
+    out, ref = _prefill(pool, new, 2)
+    _close(out, ref, "bf16", _v_max(pool))
+    pool = Pool([n + i % 3 for i, n in enumerate(new)], 1, 64, 16, "f32", seed=13)
+    out, ref = _prefill(pool, new, 2)
+    _close(out, ref, "f32", _v_max(pool))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prefill_queries_before_the_first_row_get_zeros(dtype):
+    """A length shorter than the chunk: the chunk's first queries lie before row 0 and see nothing."""
+    sa = _sa()
+    pool = Pool([40], 1, 64, 16, dtype, seed=14)
+    q = pool.q(100, 2)
+    out = sa.attn_paged_prefill(q.cuda(), pool.kp, pool.vp, pool.table, pool.kv_lens,
+                                torch.tensor([0, 100], dtype=torch.int32).cuda(), 0.125)
+    torch.cuda.synchronize()
+    assert (out[:60] == 0).all()
+    _close(out[60:], attend(q[60:], pool.k[0], pool.v[0], range(40), 0.125), dtype, _v_max(pool))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prefill_reports_bad_pages_and_token_ranges(dtype):
+    sa = _sa()
+    with sa.Context(0) as ctx:
+        pool = Pool([40, 20], 1, 64, 16, dtype, seed=8, pad_cols=0)
+        q = pool.q(10, 1).cuda()
+        bad = pool.table.clone()
+        bad[0, 1] = -7
+        good_cu = torch.tensor([0, 5, 10], dtype=torch.int32).cuda()
+        for table, lens, cu in ((bad, pool.kv_lens, good_cu), (pool.table, pool.kv_lens + 9, good_cu),
+                                (pool.table, pool.kv_lens, good_cu + 1), (pool.table, pool.kv_lens, -good_cu)):
+            sa.attn_paged_prefill(q, pool.kp, pool.vp, table, lens, cu, 1.0, ctx=ctx)
+            with pytest.raises(sa.SAError) as e:
+                ctx.synchronize()
+            assert e.value.code == -6
+        sa.attn_paged_prefill(q, pool.kp, pool.vp, pool.table, pool.kv_lens, good_cu, 1.0, ctx=ctx)
+        ctx.synchronize()
+
+
+# ---------------------------------------------------------------- shared prefix
+
+def _prefix(lens, prefix, hq, hkv, d, page, dtype, seed=0, scale=None, spread=1.0, interleaved_kv=False, ctx=None):
+    """The pool's first sequence is the prefix, the others the batch."""
+    sa = _sa()
+    pool = Pool([prefix] + list(lens), hkv, d, page, dtype, seed=seed, interleaved_kv=interleaved_kv)
+    scale = scale or 1.0 / math.sqrt(d)
+    n = len(lens)
+    q = pool.q(n, hq, spread)
+    out = sa.attn_paged_decode_prefix(q.cuda(), pool.kp, pool.vp, pool.table[0], prefix, pool.table[1:], pool.kv_lens[1:],
+                                      scale, ctx=ctx)
+    ref = torch.cat([attend(q[b:b + 1], torch.cat([pool.k[0], pool.k[b + 1]], 1), torch.cat([pool.v[0], pool.v[b + 1]], 1),
+                            [prefix + m - 1], scale) for b, m in enumerate(lens)])
+    return out, ref, _v_max(pool)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 16), (128, 128), (64, 32)])
+@pytest.mark.parametrize("hq,hkv,n", [(1, 1, 1), (4, 2, 4), (16, 2, 17), (3, 1, 90), (2, 1, 65), (16, 1, 25)])
+def test_prefix(dtype, d, page, hq, hkv, n):
+    lens = [(37 * i) % 90 for i in range(n)]               # 0 among them
+    out, ref, v_max = _prefix(lens, 333, hq, hkv, d, page, dtype, seed=n)
+    _close(out, ref, dtype, v_max)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("prefix", [0, 1, 15, 16, 64, 127, 128, 129, 256, 5000])
+def test_prefix_lengths(dtype, prefix):
+    out, ref, v_max = _prefix([0, 5, 200, 1, 64], prefix, 4, 2, 128, 16, dtype, seed=prefix)
+    _close(out, ref, dtype, v_max)
+    if prefix == 0:
+        assert (out[0] == 0).all()                         # nothing to see at all
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prefix_long_own_rows_and_large_batches(dtype):
+    out, ref, v_max = _prefix([9000, 0, 3], 700, 8, 2, 128, 16, dtype, seed=1, interleaved_kv=True)
+    _close(out, ref, dtype, v_max)
+    out, ref, v_max = _prefix([i % 5 for i in range(700)], 257, 2, 1, 64, 16, dtype, seed=2)
+    _close(out, ref, dtype, v_max)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prefix_reports_bad_pages(dtype):
+    sa = _sa()
+    with sa.Context(0) as ctx:
+        pool = Pool([40, 20], 1, 64, 16, dtype, seed=8)
+        q = pool.q(1, 1).cuda()
+        bad = pool.table[0].clone()
+        bad[2] = 1 << 20
+        sa.attn_paged_decode_prefix(q, pool.kp, pool.vp, bad, 40, pool.table[1:], pool.kv_lens[1:], 1.0, ctx=ctx)
+        with pytest.raises(sa.SAError) as e:
+            ctx.synchronize()
+        assert e.value.code == -6
+        sa.attn_paged_decode_prefix(q, pool.kp, pool.vp, pool.table[0], 40, pool.table[1:], pool.kv_lens[1:], 1.0, ctx=ctx)
+        ctx.synchronize()

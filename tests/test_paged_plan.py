@@ -32,6 +32,16 @@ int main() {
                 for (int r = t.row0(i, tk); r < t.row0(i, tk) + tk; ++r) printf(" %d", (int)t.sees(r));
             }
             printf("\n");
+        } else if (!strcmp(op, "unit")) {
+            int p0, l0, l1, w, s, tk;
+            if (scanf("%d %d %d %d %d %d", &p0, &l0, &l1, &w, &s, &tk) != 6) return 1;
+            UnitTiles u = make_unit(p0, l0, l1, w, s, tk);
+            printf("%d %d %d", u.t.n, u.n[0], u.n[1]);
+            for (int i = 0; i < u.t.n; ++i) {
+                printf(" %d", u.t.row0(i, tk));
+                for (int r = u.t.row0(i, tk); r < u.t.row0(i, tk) + tk; ++r) printf(" %d", (int)u.t.sees(r));
+            }
+            printf("\n");
         } else if (!strcmp(op, "share")) {
             long long total, n;
             if (scanf("%lld %lld", &total, &n) != 2) return 1;
@@ -92,6 +102,35 @@ def test_tiles_cover_what_is_seen_once(ask):
                 assert bool(f & 1) == any(part16) and bool(f & 2) == all(part16)
         assert rows == seen, (n, w, s, tk)
         assert starts == sorted(set(starts))
+
+
+def test_units_hold_what_their_queries_see(ask):
+    """Two slots of consecutive queries: every row that a slot's query sees lies in the slot's tiles, tiles come once
+    and in order, and a row that no query sees is not asked for unless it lies between rows of the window."""
+    rng = random.Random(2)
+    cases = []
+    for _ in range(400):
+        n0, n1 = rng.randint(1, 40), rng.randint(0, 40)
+        p0 = rng.choice([0, 0, rng.randint(-60, 400)])
+        last0 = max(-1, p0 + n0 - 1)
+        last1 = max(-1, p0 + n0 + n1 - 1) if n1 else -1
+        cases.append((p0, last0, last1, rng.choice([0, 1, 30, 64, 200]), rng.choice([0, 1, 4, 64, 100]),
+                      rng.choice([16, 64, 128]), n0, n1))
+    for (p0, last0, last1, w, s, tk, n0, n1), got in zip(cases, ask("unit %d %d %d %d %d %d" % c[:6] for c in cases)):
+        n = got[:3]
+        per = 1 + tk
+        tiles = [got[3 + i * per:3 + (i + 1) * per] for i in range(n[0])]
+        starts = [x[0] for x in tiles]
+        assert starts == sorted(set(starts)) and all(x % tk == 0 for x in starts) and n[0] == max(n[1:])
+        asked = {x[0] + i for x in tiles for i, f in enumerate(x[1:]) if f}
+        for slot, (a, b) in enumerate(((p0, p0 + n0), (p0 + n0, p0 + n0 + n1))):
+            mine = {x + i for x in starts[:n[1 + slot]] for i in range(tk)}
+            for p in range(a, b):
+                seen = {j for j in range(max(0, p + 1)) if sees(p, j, w, s)}
+                assert seen <= mine and seen <= asked
+        top = max(last0, last1)
+        lo = max(0, max(p0, 0) - w + 1) if w else 0
+        assert all(j <= top and (j >= lo or j < s) for j in asked)
 
 
 def test_tiles_of_the_longest_sequences(ask):
