@@ -39,7 +39,7 @@ class PagedKV(C.Structure):
                 ("table_stride", C.c_longlong), ("max_pages", C.c_int), ("kv_lens", _vp), ("n_seqs", C.c_int)]
 
 
-_kvp = C.POINTER(PagedKV)
+_kvp = C.c_void_p      # const sa_paged_kv*: byref(PagedKV(...)) or the packed bytes
 _szp = C.POINTER(C.c_size_t)
 
 # (name, restype, argtypes) for every entry point of include/sa_cuda.h

@@ -152,3 +152,10 @@ def test_python_wrappers_refuse_host_tensors_and_wrong_shapes():
     meta = torch.zeros(4, 2, 16, 64, device="meta")
     with pytest.raises(ValueError, match="CUDA"):
         sa.paged_append(torch.zeros(1, 2, 64), torch.zeros(1, 2, 64), meta, meta, table, lens)
+
+
+def test_packed_description_is_the_struct():
+    from streaming_attention_b200.paged import _pack
+    kv = _kv(k_pages=1 << 40, v_pages=3 << 40, page_stride=1 << 35, table_stride=7, n_seqs=9)
+    vals = [getattr(kv, f) for f, _ in PagedKV._fields_]
+    assert bytes(kv)[:len(_pack(*vals))] == _pack(*vals) and C.sizeof(kv) - len(_pack(*vals)) < 8
