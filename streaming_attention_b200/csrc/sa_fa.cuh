@@ -107,5 +107,56 @@ __device__ __forceinline__ float emit_p(const float* sc, float sl2, float nm, ui
     return (ps[0] + ps[1]) + (ps[2] + ps[3]);
 }
 
+// emit_p with the scale and the row sum on packed fp32 pairs (fma/add.f32x2:
+// half the FMA-pipe instructions; each element rounds as in emit_p, the sum's
+// order differs).
+__device__ __forceinline__ unsigned long long f2(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void un2(unsigned long long r, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+template <bool TRACK_MAX>
+__device__ __forceinline__ float emit_p2(const float* sc, float sl2, float nm, uint32_t p_addr, float* mx_out) {
+    const unsigned long long s2 = f2(sl2, sl2), n2 = f2(nm, nm);
+    unsigned long long ps[4] = {0ull, 0ull, 0ull, 0ull};
+    float mx[4];
+    if constexpr (TRACK_MAX) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = sc[i];
+    }
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int c = hf * 64; c < hf * 64 + 64; c += 2) {
+            if constexpr (TRACK_MAX) mx[(c >> 1) & 3] = fmaxf(fmaxf(mx[(c >> 1) & 3], sc[c]), sc[c + 1]);
+            float e0, e1;
+            un2(fma2(f2(sc[c], sc[c + 1]), s2, n2), e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            ps[(c >> 1) & 3] = add2(ps[(c >> 1) & 3], f2(e0, e1));
+            pk[(c >> 1) & 31] = pack_bf16(e0, e1);
+        }
+        tc::tmem_st32(p_addr + hf * 32, pk);
+    }
+    if constexpr (TRACK_MAX) *mx_out = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    float a, b;
+    un2(add2(add2(ps[0], ps[1]), add2(ps[2], ps[3])), a, b);
+    return a + b;
+}
+
 }  // namespace pf
 }  // namespace sa

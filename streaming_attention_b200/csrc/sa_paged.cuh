@@ -3,6 +3,7 @@
 // window with first tokens that stay visible, and the host-side checks.
 #pragma once
 #include <cuda.h>
+#include <cuda_bf16.h>
 #include <cstdint>
 
 #include "sa_internal.h"
@@ -42,6 +43,85 @@ __device__ __forceinline__ int checked_page(const Cache& c, int entry) {
     atomicExch(c.status, SA_STATUS_BAD_INDEX);
     return -1;
 }
+
+// One warp joins partial softmax states of one query row, lane by lane D / 32
+// columns: m = max m_i, l = sum 2^(m_i - m) l_i, O = sum 2^(m_i - m) O_i.
+// 32 parts at a time: the lanes fetch their (m, l), then the O rows are read
+// eight at once, with nothing between the loads that waits for one of them.
+template <int D>
+struct Joined {
+    static constexpr int V = D / 32;
+    float m, l, o[V];                  // l: this lane's share, see total()
+    __device__ __forceinline__ Joined() : m(-INFINITY), l(0.f) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = 0.f;
+    }
+    // ml(p) -> (m, l) of part p;  row(p) -> its O row
+    template <typename ML, typename ROW>
+    __device__ __forceinline__ void add(int parts, int lane, ML ml, ROW row) {
+        for (int base = 0; base < parts; base += 32) {
+            float2 x = make_float2(-INFINITY, 0.f);
+            if (base + lane < parts) x = ml(base + lane);
+            float mx = x.x;
+#pragma unroll
+            for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+            const float M = fmaxf(m, mx);
+            if (M == -INFINITY) continue;
+            const float corr = ex2(m - M), w = ex2(x.x - M);        // 0 for an empty state
+            m = M;
+            l = l * corr + w * x.y;
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] *= corr;
+            const int n = min(32, parts - base);
+            for (int i0 = 0; i0 < n; i0 += 8) {
+                float v[8][V], wi[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    wi[i] = __shfl_sync(0xffffffffu, w, (i0 + i) & 31);
+                    const bool on = i0 + i < n && wi[i] > 0.f;      // the O of an empty part is not written
+                    const float* r = on ? row(base + i0 + i) + lane * V : nullptr;
+                    if (!on) wi[i] = 0.f;
+                    if constexpr (V == 2) {
+                        const float2 y = on ? *reinterpret_cast<const float2*>(r) : make_float2(0.f, 0.f);
+                        v[i][0] = y.x; v[i][1] = y.y;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < V; c += 4) {
+                            const float4 y = on ? *reinterpret_cast<const float4*>(r + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            v[i][c] = y.x; v[i][c + 1] = y.y; v[i][c + 2] = y.z; v[i][c + 3] = y.w;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) o[e] = fmaf(wi[i], v[i][e], o[e]);
+            }
+        }
+    }
+    __device__ __forceinline__ float total() const {
+        float t = l;
+#pragma unroll
+        for (int off = 16; off; off >>= 1) t += __shfl_xor_sync(0xffffffffu, t, off);
+        return t;
+    }
+    // The lane's columns of the normalised row (NaN after an expired wait), in OT.
+    template <typename OT>
+    __device__ __forceinline__ void store(OT* dst, int lane, const int* status) const {
+        const float t = total();
+        const bool failed = *reinterpret_cast<const volatile int*>(status) == SA_STATUS_TIMEOUT;
+        const float f = failed ? nanf("") : (t > 0.f ? 1.f / t : 0.f);
+        dst += lane * V;
+        if constexpr (sizeof(OT) == 4) {
+#pragma unroll
+            for (int e = 0; e < V; e += 2) *reinterpret_cast<float2*>(dst + e) = make_float2(o[e] * f, o[e + 1] * f);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e += 2)
+                *reinterpret_cast<__nv_bfloat162*>(dst + e) = __floats2bfloat162_rn(o[e] * f, o[e + 1] * f);
+        }
+    }
+};
 
 // The tokens of a ragged batch cut into units of up to `per` tokens of one
 // sequence, numbered over the batch.

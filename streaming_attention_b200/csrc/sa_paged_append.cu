@@ -29,23 +29,37 @@ struct AppendArgs {
     const int* cu_q;                     // null: one token per sequence
     const float *cos_t, *sin_t;          // [n_pos][R/2], null: no rotation
     int n_pos, rot, interleaved;
-    int n_tokens, hq, d, pos0;
+    int n_tokens, hq, d, pos0, head_log2;
 };
 
-template <typename T> __device__ __forceinline__ void load8(const T* p, float* f);
-template <> __device__ __forceinline__ void load8<float>(const float* p, float* f) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float* f) {
-    const uint4 r = __ldcs(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+// Eight elements as they lie in memory.
+template <typename T> struct Raw8 {
+    static constexpr int N = sizeof(T) / 2;
+    uint4 w[N];
+    __device__ __forceinline__ void load(const T* p) {       // read once
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        for (int i = 0; i < N; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
     }
+    __device__ __forceinline__ void floats(float* f) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (N == 2) {
+                    f[4 * i + j] = __uint_as_float(v[j]);
+                } else {
+                    f[2 * j] = __uint_as_float(v[j] << 16);
+                    f[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
+                }
+            }
+        }
+    }
+};
+// table rows are shared by a token's heads: kept in the cache
+__device__ __forceinline__ void load4t(const float* p, float* f) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
 }
 template <typename T> __device__ __forceinline__ void store8(T* p, const float* f);
 template <> __device__ __forceinline__ void store8<float>(float* p, const float* f) {
@@ -69,31 +83,39 @@ struct Place {
 };
 
 // One warp finds a token's sequence: the number of starts cu_q[1..] at or
-// before it, 32 at a time.
+// before it, 32 sequences at a time; the lane of the sequence has its length
+// and first token in hand.
 __device__ __forceinline__ Place find_place(const AppendArgs& a, int tok, int lane) {
     Place p;
     p.pos = 0;
     p.page = -1;
     p.row = 0;
-    int b = tok, t = 0, n = 1;
+    int b = tok, t = 0, n = 1, len = 0;
     if (a.cu_q) {
         b = 0;
         for (int base = 0; base < a.c.n_seqs; base += 32) {
             const int i = base + lane;
-            const bool at = i < a.c.n_seqs && a.cu_q[i + 1] <= tok;
-            const int got = __popc(__ballot_sync(0xffffffffu, at));
+            int c0 = 0, c1 = 0x7fffffff, l = 0;
+            if (i < a.c.n_seqs) {
+                c0 = a.cu_q[i];
+                c1 = a.cu_q[i + 1];
+                l = a.c.kv_lens[i];
+            }
+            const int got = __popc(__ballot_sync(0xffffffffu, c1 <= tok));
             b += got;
-            if (got < 32) break;
-        }
-        if (b < a.c.n_seqs) {
-            const int c0 = a.cu_q[b];
+            if (got == 32) continue;
+            c0 = __shfl_sync(0xffffffffu, c0, got);
+            n = __shfl_sync(0xffffffffu, c1, got) - c0;
+            len = __shfl_sync(0xffffffffu, l, got);
             t = tok - c0;
-            n = a.cu_q[b + 1] - c0;
+            break;
         }
     }
     if (b >= a.c.n_seqs || t < 0) return p;              // a row of no sequence
-    const int len = a.c.kv_lens[b];
-    if (len <= 0 && !a.cu_q) return p;                   // an empty slot of a padded batch
+    if (!a.cu_q) {
+        len = a.c.kv_lens[b];
+        if (len <= 0) return p;                          // an empty slot of a padded batch
+    }
     const long long at = append_row(len, n, t, a.c.max_pages, a.c.page_log2, a.pos0, a.cos_t ? a.n_pos : 1LL << 40);
     if (at < 0) {
         if (lane == 0) atomicExch(a.c.status, SA_STATUS_BAD_INDEX);
@@ -105,86 +127,107 @@ __device__ __forceinline__ Place find_place(const AppendArgs& a, int tok, int la
     return p;
 }
 
-// One CTA per token.  A thread moves two groups of eight elements of one head
-// at a time: the two halves of eight rotated pairs, or two neighbouring groups.
-template <typename T, typename KT>
-__global__ void __launch_bounds__(AT) append_kernel(const AppendArgs a) {
-    __shared__ Place s_place;
-    const int tok = blockIdx.x, tid = threadIdx.x;
-    const int per_head = a.d / 16;                       // thread items per head
-    const int heads = (a.q ? a.hq : 0) + 2 * a.c.hkv;
-    const int nq = a.q ? a.hq : 0;
-    const int rot_items = a.rot / 16;
-    const int items = heads * per_head;
-    bool ready = false;
+// WPT warps per token, each by itself: it looks up the token's place while its
+// first rows are on their way.  A lane moves items of two groups of eight
+// elements of one head, half the rotated part (or half the rest) apart: the two
+// halves of eight rotated pairs.  A head has d / 16 items, so a lane's item is
+// the same one of every head it meets and its angles are fetched once.
+template <typename T, typename KT, int WPT, int U>
+__global__ void __launch_bounds__(AT, 2) append_kernel(const AppendArgs a) {
+    const int lane = threadIdx.x & 31;
+    const long long w = (long long)blockIdx.x * (AT / 32) + (threadIdx.x >> 5);
+    const long long tok = w / WPT;
+    if (tok >= a.n_tokens) return;
+    const int head_log2 = a.head_log2;
+    const int nq = a.q ? a.hq : 0, nk = nq + a.c.hkv;
+    const int items = (nk + a.c.hkv) << head_log2;
+    const int g = lane & ((1 << head_log2) - 1);
+    const bool turns = g < a.rot / 16;
+    // where the item lies in a head that is rotated, and in one that is not
+    const int r0 = turns ? g * 8 : a.rot + (g - a.rot / 16) * 8, r1 = r0 + (turns ? a.rot : a.d - a.rot) / 2;
+    const int v0 = g * 8, v1 = v0 + a.d / 2;
+    float c[8], s[8];
+    bool found = false;
     Place pl;
-    for (int it = tid; it < items || !ready; it += AT) {
-        float x[8], y[8];
-        int h = 0, g = 0, o0 = 0, o1 = 0;
-        const bool on = it < items;
-        if (on) {
-            h = it / per_head;
-            g = it - h * per_head;
-            const bool turn = h < nq + a.c.hkv;
-            const bool split = turn && !a.interleaved && g < rot_items;
-            o0 = split ? g * 8 : g * 16;
-            o1 = split ? o0 + a.rot / 2 : o0 + 8;
-            const T* src = h < nq ? static_cast<const T*>(a.q) + (long long)tok * a.q_stride + (long long)h * a.d
-                           : h < nq + a.c.hkv
-                               ? static_cast<const T*>(a.k) + (long long)tok * a.k_stride + (long long)(h - nq) * a.d
-                               : static_cast<const T*>(a.v) + (long long)tok * a.v_stride +
-                                     (long long)(h - nq - a.c.hkv) * a.d;
-            load8<T>(src + o0, x);
-            load8<T>(src + o1, y);
-        }
-        if (!ready) {                                     // the rows are on their way while the place is looked up
-            if (tid < 32) {
-                const Place p = find_place(a, tok, tid);
-                if (tid == 0) s_place = p;
+    for (int base = (int)(w % WPT) * 32; base < items; base += U * WPT * 32) {
+        Raw8<T> x[U], y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int it = base + u * WPT * 32 + lane, h = it >> head_log2;
+            if (it < items) {
+                const T* src = h < nq   ? static_cast<const T*>(a.q) + tok * a.q_stride + (long long)h * a.d
+                               : h < nk ? static_cast<const T*>(a.k) + tok * a.k_stride + (long long)(h - nq) * a.d
+                                        : static_cast<const T*>(a.v) + tok * a.v_stride + (long long)(h - nk) * a.d;
+                x[u].load(src + (h < nk ? r0 : v0));
+                y[u].load(src + (h < nk ? r1 : v1));
             }
-            __syncthreads();
-            pl = s_place;
-            ready = true;
         }
-        if (!on || pl.page < 0) break;
-        if (h < nq + a.c.hkv && g < rot_items) {
-            const long long r = (long long)pl.pos * (a.rot / 2);
-            if (a.interleaved) {                          // eight pairs lie in x then y
-                float c[8], s[8];
-                load8<float>(a.cos_t + r + g * 8, c);
-                load8<float>(a.sin_t + r + g * 8, s);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float xa = x[2 * i], xb = x[2 * i + 1], ya = y[2 * i], yb = y[2 * i + 1];
-                    x[2 * i] = xa * c[i] - xb * s[i];
-                    x[2 * i + 1] = xb * c[i] + xa * s[i];
-                    y[2 * i] = ya * c[4 + i] - yb * s[4 + i];
-                    y[2 * i + 1] = yb * c[4 + i] + ya * s[4 + i];
-                }
-            } else {
-                float c[8], s[8];
-                load8<float>(a.cos_t + r + o0, c);
-                load8<float>(a.sin_t + r + o0, s);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float u = x[i], w = y[i];
-                    x[i] = u * c[i] - w * s[i];
-                    y[i] = w * c[i] + u * s[i];
+        if (!found) {
+            pl = find_place(a, (int)tok, lane);
+            if (pl.page < 0) return;
+            found = true;
+            if (turns) {
+                const long long r = (long long)pl.pos * (a.rot / 2);
+                if (a.interleaved) {                      // four pairs in each group
+                    load4t(a.cos_t + r + g * 4, c);
+                    load4t(a.sin_t + r + g * 4, s);
+                    load4t(a.cos_t + r + a.rot / 4 + g * 4, c + 4);
+                    load4t(a.sin_t + r + a.rot / 4 + g * 4, s + 4);
+                } else {
+                    load4t(a.cos_t + r + g * 8, c);
+                    load4t(a.sin_t + r + g * 8, s);
+                    load4t(a.cos_t + r + g * 8 + 4, c + 4);
+                    load4t(a.sin_t + r + g * 8 + 4, s + 4);
                 }
             }
         }
-        KT* dst;
-        if (h < nq) {
-            dst = static_cast<KT*>(a.q_out) + (long long)tok * a.qo_stride + (long long)h * a.d;
-        } else {
-            const bool key = h < nq + a.c.hkv;
-            const int kh = key ? h - nq : h - nq - a.c.hkv;
-            dst = reinterpret_cast<KT*>(key ? a.c.k : a.c.v) + (long long)pl.page * a.c.page_stride +
-                  (((long long)kh << a.c.page_log2) + pl.row) * a.d;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int it = base + i * WPT * 32 + lane, h = it >> head_log2;
+            if (it >= items) continue;
+            float u[8], v[8];
+            x[i].floats(u);
+            y[i].floats(v);
+            if (h < nk && turns) {
+                if (a.interleaved) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float ua = u[2 * e], ub = u[2 * e + 1], va = v[2 * e], vb = v[2 * e + 1];
+                        u[2 * e] = ua * c[e] - ub * s[e];
+                        u[2 * e + 1] = ub * c[e] + ua * s[e];
+                        v[2 * e] = va * c[4 + e] - vb * s[4 + e];
+                        v[2 * e + 1] = vb * c[4 + e] + va * s[4 + e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float p = u[e], q = v[e];
+                        u[e] = p * c[e] - q * s[e];
+                        v[e] = q * c[e] + p * s[e];
+                    }
+                }
+            }
+            KT* dst = h < nq ? static_cast<KT*>(a.q_out) + tok * a.qo_stride + (long long)h * a.d
+                             : reinterpret_cast<KT*>(h < nk ? a.c.k : a.c.v) + (long long)pl.page * a.c.page_stride +
+                                   (((long long)(h < nk ? h - nq : h - nk) << a.c.page_log2) + pl.row) * a.d;
+            store8<KT>(dst + (h < nk ? r0 : v0), u);
+            store8<KT>(dst + (h < nk ? r1 : v1), v);
         }
-        store8<KT>(dst + o0, x);
-        store8<KT>(dst + o1, y);
     }
+}
+
+template <typename T, typename KT>
+static int append_launch(cudaStream_t st, int num_sms, const AppendArgs& a) {
+    // A warp per token with four items in flight where that fills the GPU (8418
+    // tokens of 16/8 heads of 128 bf16: 28.2 us against 35-44 of a CTA per token,
+    // which looks every token's place up eight times); below, a CTA per token
+    // spreads the rows over more SMs (8 tokens: 2.5 us against 5.6).
+    if (a.n_tokens >= 16 * num_sms)
+        append_kernel<T, KT, 1, 4><<<(a.n_tokens + AT / 32 - 1) / (AT / 32), AT, 0, st>>>(a);
+    else
+        append_kernel<T, KT, AT / 32, 1><<<a.n_tokens, AT, 0, st>>>(a);
+    SA_CUDA_TRY(cudaGetLastError());
+    return SA_OK;
 }
 
 // cos / sin [n_pos][R/2] of p * theta^(-2i/R): angles in 64 bits (a far
@@ -261,10 +304,11 @@ SA_API int sa_paged_append(sa_ctx* ctx, const sa_paged_kv* kv, int x_dtype, cons
     a.cos_t = cos_t; a.sin_t = sin_t;
     a.n_pos = n_pos; a.rot = cos_t ? rotary_dim : 0; a.interleaved = interleaved ? 1 : 0;
     a.n_tokens = n_tokens; a.hq = hq; a.d = d; a.pos0 = pos0;
+    a.head_log2 = pg::log2_exact(d / 16);
     const bool xf = x_dtype == SA_F32, cf = kv->dtype == SA_F32;
-    auto kern = xf ? (cf ? pg::append_kernel<float, float> : pg::append_kernel<float, __nv_bfloat16>)
-                   : (cf ? pg::append_kernel<__nv_bfloat16, float> : pg::append_kernel<__nv_bfloat16, __nv_bfloat16>);
-    kern<<<n_tokens, pg::AT, 0, ctx->stream>>>(a);
-    SA_CUDA_TRY(cudaGetLastError());
-    return SA_OK;
+    using bf = __nv_bfloat16;
+    if (xf) return cf ? pg::append_launch<float, float>(ctx->stream, ctx->num_sms, a)
+                      : pg::append_launch<float, bf>(ctx->stream, ctx->num_sms, a);
+    return cf ? pg::append_launch<bf, float>(ctx->stream, ctx->num_sms, a)
+              : pg::append_launch<bf, bf>(ctx->stream, ctx->num_sms, a);
 }

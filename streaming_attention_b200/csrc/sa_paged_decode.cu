@@ -288,6 +288,13 @@ __device__ __forceinline__ void drain(Ring* r) {
     __syncthreads();
 }
 
+// Behind a shared prefix the launch starts while the prefix's kernel still runs
+// (neither reads what the other writes); it ends only after that kernel, so that
+// the join, which waits for this one, has both.
+__device__ __forceinline__ void leave(const DecodeArgs& a) {
+    if (a.to_state) pdl_wait();
+}
+
 // ---- bf16 -------------------------------------------------------------------
 constexpr int BW = 4;                        // consumer warps
 constexpr int BTHREADS = (BW + 1) * 32;
@@ -353,7 +360,10 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     }
     plan_share<BTHREADS>(a, TK, &r.share, r.scan);
     const Share sh = r.share;
-    if (sh.count == 0) return;
+    if (sh.count == 0) {
+        leave(a);
+        return;
+    }
     if (tid == 0) r.consumed = sh.count;
     Walk w;
     w.b = sh.b; w.h = sh.h; w.i = sh.i; w.left = sh.count;
@@ -363,6 +373,7 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     if (warp == BW) {
         produce<__nv_bfloat16, D>(&tk, &tv, a, &r, buf, w, lane);
         drain(&r);
+        leave(a);
         return;
     }
     const int qc = lane >> 2, qp = (lane & 3) * 2;      // column as operand; first of two columns as accumulator
@@ -521,17 +532,15 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                         dst[d * 16 + 8] = __float2bfloat16_rn(o[n][d][2 + j] * inv);
                     }
                 } else {
-                    float* dst = (ds.kind == TO_STATE ? a.ws.state : a.ws.slots) +
-                                 ((long long)ds.slot * a.G + g) * (D + 2);
+                    const long long at = (long long)ds.slot * a.G + g;
+                    float* dst = (ds.kind == TO_STATE ? a.ws.state_o : a.ws.slot_o) + at * D;
 #pragma unroll
                     for (int d = 0; d < D / 16; ++d) {
                         dst[d * 16 + qc] = o[n][d][j];
                         dst[d * 16 + 8 + qc] = o[n][d][2 + j];
                     }
-                    if (qc == 0) {
-                        dst[D] = m[n][j];
-                        dst[D + 1] = l[n][j];
-                    }
+                    if (qc == 0)
+                        (ds.kind == TO_STATE ? a.ws.state_ml : a.ws.slot_ml)[at] = make_float2(m[n][j], l[n][j]);
                 }
             }
         }
@@ -539,6 +548,7 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     }
     if (!ok && lane == 0) atomicMin(&r.consumed, it);
     drain(&r);
+    leave(a);
 }
 
 // ---- fp32 -------------------------------------------------------------------
@@ -580,7 +590,10 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
     }
     plan_share<THREADS>(a, TK, &r.share, r.scan);
     const Share sh = r.share;
-    if (sh.count == 0) return;
+    if (sh.count == 0) {
+        leave(a);
+        return;
+    }
     if (tid == 0) r.consumed = sh.count;
     Walk w;
     w.b = sh.b; w.h = sh.h; w.i = sh.i; w.left = sh.count;
@@ -590,6 +603,7 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
     if (warp == NW) {
         produce<float, D>(nullptr, nullptr, a, &r, buf, w, lane);
         drain(&r);
+        leave(a);
         return;
     }
     const int grp = lane >> 3, sub = lane & 7, part = warp & 3, g0 = (warp >> 2) * HG;
@@ -742,50 +756,40 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
                 static_cast<float*>(a.out)[(long long)b * a.o_stride + (long long)(h * a.G + g) * D + col] =
                     L > 0.f ? O / L : 0.f;
             } else {
-                float* dst = (ds.kind == TO_STATE ? a.ws.state : a.ws.slots) + ((long long)ds.slot * a.G + g) * (D + 2);
-                dst[col] = O;
-                if (col == 0) {
-                    dst[D] = M;
-                    dst[D + 1] = L;
-                }
+                const long long at = (long long)ds.slot * a.G + g;
+                (ds.kind == TO_STATE ? a.ws.state_o : a.ws.slot_o)[at * D + col] = O;
+                if (col == 0) (ds.kind == TO_STATE ? a.ws.state_ml : a.ws.slot_ml)[at] = make_float2(M, L);
             }
         }
         bar_consumers<NW * 32>();
     }
     if (!ok && lane == 0) atomicMin(&r.consumed, it);
     drain(&r);
+    leave(a);
 }
 
 // ---- the join ----------------------------------------------------------------
 // CTA c joins the shares of the pair whose first tile CTA c of the decode held
-// and whose last one it did not, if there is such a pair.
-template <typename OT>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ DecodeArgs a) {
+// and whose last one it did not, if there is such a pair; a warp per query head.
+constexpr int JW = 4;
+template <typename OT, int D>
+__global__ void __launch_bounds__(JW * 32) join_kernel(const __grid_constant__ DecodeArgs a) {
     pdl_wait();
     const int4 rec = a.ws.head[blockIdx.x];
     if (rec.x < 0) return;
-    const int D = a.ws.d, RW = D + 2;
+    const int lane = threadIdx.x & 31;
     const int b = rec.w / a.c.hkv, h = rec.w - b * a.c.hkv;
-    const int n = rec.y - rec.x + 1;
-    for (int idx = threadIdx.x; idx < a.G * D; idx += blockDim.x) {
-        const int g = idx / D, col = idx - g * D;
-        float M = -INFINITY, L = 0.f, O = 0.f;
-        for (int i = 0; i < n; ++i) {
-            const int slot = 2 * (rec.x + i) + (i == 0 ? rec.z : 0);
-            const float* s = a.ws.slots + ((long long)slot * a.G + g) * RW;
-            const float m2 = s[D], l2 = s[D + 1], o2 = s[col];
-            const float N = fmaxf(M, m2);
-            const float wa = M == -INFINITY ? 0.f : ex2(M - N), wb = m2 == -INFINITY ? 0.f : ex2(m2 - N);
-            M = N;
-            L = L * wa + l2 * wb;
-            O = O * wa + o2 * wb;
-        }
-        const bool failed = *reinterpret_cast<volatile int*>(a.c.status) == SA_STATUS_TIMEOUT;
-        const float x = failed ? nanf("") : (L > 0.f ? O / L : 0.f);
-        const long long at = (long long)b * a.o_stride + (long long)(h * a.G + g) * D + col;
-        if constexpr (sizeof(OT) == 4) static_cast<float*>(a.out)[at] = x;
-        else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(x);
+    for (int g = threadIdx.x >> 5; g < a.G; g += JW) {
+        auto at = [&](int p) { return (2LL * (rec.x + p) + (p == 0 ? rec.z : 0)) * a.G + g; };
+        Joined<D> s;
+        s.add(rec.y - rec.x + 1, lane, [&](int p) { return a.ws.slot_ml[at(p)]; },
+              [&](int p) { return a.ws.slot_o + at(p) * D; });
+        s.store(static_cast<OT*>(a.out) + (long long)b * a.o_stride + (long long)(h * a.G + g) * D, lane, a.c.status);
     }
+}
+template <typename OT>
+static auto join_pick(int d) {
+    return d == 64 ? join_kernel<OT, 64> : d == 128 ? join_kernel<OT, 128> : join_kernel<OT, 256>;
 }
 
 using F32Fn = void (*)(const DecodeArgs);
@@ -828,8 +832,12 @@ static int launch_bf16(cudaStream_t st, int grid, const CUtensorMap& tk, const C
     auto two = decode_bf16_kernel<D, (D < 256 ? 2 : 1)>;
     auto k = a.G <= 8 ? one : two;
     SA_RC_TRY(set_smem_attr_once((const void*)k, bf16_smem<D>()));
-    k<<<grid, BTHREADS, bf16_smem<D>(), st>>>(tk, tv, a);
-    SA_CUDA_TRY(cudaGetLastError());
+    if (a.to_state) {
+        SA_CUDA_TRY(launch_pdl(k, dim3(grid), dim3(BTHREADS), bf16_smem<D>(), st, tk, tv, a));
+    } else {
+        k<<<grid, BTHREADS, bf16_smem<D>(), st>>>(tk, tv, a);
+        SA_CUDA_TRY(cudaGetLastError());
+    }
     return SA_OK;
 }
 
@@ -853,8 +861,12 @@ int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q
     if (kv->dtype == SA_F32) {
         const F32Pick p = f32_pick_d(kv->d, a.G);
         SA_RC_TRY(set_smem_attr_once((const void*)p.fn, p.smem));
-        p.fn<<<grid, p.threads, p.smem, st>>>(a);
-        SA_CUDA_TRY(cudaGetLastError());
+        if (to_state) {
+            SA_CUDA_TRY(launch_pdl(p.fn, dim3(grid), dim3(p.threads), p.smem, st, a));
+        } else {
+            p.fn<<<grid, p.threads, p.smem, st>>>(a);
+            SA_CUDA_TRY(cudaGetLastError());
+        }
     } else {
         CUtensorMap tk, tv;
         const int tile = kv->d == 64 ? Geo<__nv_bfloat16, 64>::TK : Geo<__nv_bfloat16, 128>::TK;
@@ -866,14 +878,14 @@ int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q
                                  : launch_bf16<256>(st, grid, tk, tv, a));
     }
     if (to_state) return SA_OK;
-    if (kv->dtype == SA_F32) SA_CUDA_TRY(launch_pdl(join_kernel<float>, dim3(grid), dim3(128), 0, st, a));
-    else SA_CUDA_TRY(launch_pdl(join_kernel<__nv_bfloat16>, dim3(grid), dim3(128), 0, st, a));
+    auto join = kv->dtype == SA_F32 ? join_pick<float>(kv->d) : join_pick<__nv_bfloat16>(kv->d);
+    SA_CUDA_TRY(launch_pdl(join, dim3(grid), dim3(JW * 32), 0, st, a));
     return SA_OK;
 }
 
 size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool to_state, void* base, DecodeWs* ws) {
     const int grid = decode_grid(ctx, kv, hq), G = hq / kv->hkv;
-    const size_t row = (size_t)(kv->d + 2) * 4;
+    const size_t slots = (size_t)grid * 2 * G, rows = (size_t)kv->n_seqs * hq, d4 = (size_t)kv->d * 4;
     size_t at = 0;
     unsigned char* p = static_cast<unsigned char*>(base);
     auto take = [&](size_t bytes) {
@@ -882,10 +894,12 @@ size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool t
         return p ? p + o : nullptr;
     };
     DecodeWs w = {};
-    w.slots = reinterpret_cast<float*>(take((size_t)grid * 2 * G * row));
+    w.slot_o = reinterpret_cast<float*>(take(slots * d4));
+    w.slot_ml = reinterpret_cast<float2*>(take(slots * 8));
     if (to_state) {
         w.pair = reinterpret_cast<int4*>(take((size_t)kv->n_seqs * kv->hkv * sizeof(int4)));
-        w.state = reinterpret_cast<float*>(take((size_t)kv->n_seqs * hq * row));
+        w.state_o = reinterpret_cast<float*>(take(rows * d4));
+        w.state_ml = reinterpret_cast<float2*>(take(rows * 8));
     } else {
         w.head = reinterpret_cast<int4*>(take((size_t)grid * sizeof(int4)));
     }

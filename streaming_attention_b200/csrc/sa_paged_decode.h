@@ -6,13 +6,15 @@
 namespace sa {
 namespace pg {
 
-// Shares of (sequence, KV head) pairs that several CTAs hold.  States are rows
-// of d + 2 floats: the unnormalised O, then m (log2 domain) and l.
+// Shares of (sequence, KV head) pairs that several CTAs hold: unnormalised O
+// rows of d floats and (m in the log2 domain, l).
 struct DecodeWs {
-    float* slots;     // [grid][2][G]: the first and the last pair of a CTA
+    float* slot_o;    // [grid][2][G][d]: the first and the last pair of a CTA
+    float2* slot_ml;  // [grid][2][G]
     int4* head;       // [grid]: first CTA, last CTA, first CTA's slot, pair; first CTA -1: nothing to join
     int4* pair;       // [n_seqs * hkv] the same by pair (first CTA -1: the state is whole), with `state`
-    float* state;     // [n_seqs][hq]
+    float* state_o;   // [n_seqs][hq][d]
+    float2* state_ml; // [n_seqs][hq]
     int d, out_elt;
 };
 

@@ -30,65 +30,29 @@ struct JoinArgs {
     const float* part_ml;
 };
 
-struct Acc {
-    float m, l, o[4];
-    __device__ __forceinline__ void add(float m2, float l2, float4 o2) {
-        const float M = fmaxf(m, m2);
-        const float wa = m == -INFINITY ? 0.f : ex2(m - M), wb = m2 == -INFINITY ? 0.f : ex2(m2 - M);
-        m = M;
-        l = l * wa + l2 * wb;
-        o[0] = o[0] * wa + o2.x * wb;
-        o[1] = o[1] * wa + o2.y * wb;
-        o[2] = o[2] * wa + o2.z * wb;
-        o[3] = o[3] * wa + o2.w * wb;
-    }
-};
-
-// D / 4 threads per (sequence, query head).
+// A warp per (sequence, query head).
 template <typename OT, int D>
 __global__ void __launch_bounds__(JT) prefix_join_kernel(const __grid_constant__ JoinArgs a) {
     pdl_wait();
-    constexpr int TPR = D / 4;
-    const long long row = (long long)blockIdx.x * (JT / TPR) + threadIdx.x / TPR;
-    const int c4 = (threadIdx.x % TPR) * 4;
+    const int lane = threadIdx.x & 31;
+    const long long row = (long long)blockIdx.x * (JT / 32) + (threadIdx.x >> 5);
     const long long rows = (long long)a.c.n_seqs * a.hq;
     if (row >= rows) return;
     const int b = (int)(row / a.hq), h = (int)(row - (long long)b * a.hq), kvh = h / a.G, g = h - kvh * a.G;
-    Acc s;
-    s.m = -INFINITY;
-    s.l = s.o[0] = s.o[1] = s.o[2] = s.o[3] = 0.f;
-    const int parts = b >= a.alt_from ? 2 * a.n_split : a.n_split;
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-        const long long at = (long long)p * rows + row;
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-        // an empty part has no O
-        if (ml.x != -INFINITY) s.add(ml.x, ml.y, *reinterpret_cast<const float4*>(a.part_o + at * D + c4));
+    const bool own = seq_len(a.c, b) > 0;
+    const int4 rec = own ? a.ws.pair[b * a.c.hkv + kvh] : make_int4(-1, 0, 0, 0);
+    Joined<D> s;
+    s.add(b >= a.alt_from ? 2 * a.n_split : a.n_split, lane,
+          [&](int p) { return reinterpret_cast<const float2*>(a.part_ml)[p * rows + row]; },
+          [&](int p) { return a.part_o + (p * rows + row) * D; });
+    if (own && rec.x < 0)
+        s.add(1, lane, [&](int) { return a.ws.state_ml[row]; }, [&](int) { return a.ws.state_o + row * D; });
+    if (own && rec.x >= 0) {
+        auto at = [&](int p) { return (2LL * (rec.x + p) + (p == 0 ? rec.z : 0)) * a.G + g; };
+        s.add(rec.y - rec.x + 1, lane, [&](int p) { return a.ws.slot_ml[at(p)]; },
+              [&](int p) { return a.ws.slot_o + at(p) * D; });
     }
-    if (seq_len(a.c, b) > 0) {
-        const int4 rec = a.ws.pair[b * a.c.hkv + kvh];
-        const int n = rec.x < 0 ? 1 : rec.y - rec.x + 1;
-        for (int i = 0; i < n; ++i) {
-            const float* st = rec.x < 0 ? a.ws.state + row * (D + 2)
-                                        : a.ws.slots + ((2LL * (rec.x + i) + (i == 0 ? rec.z : 0)) * a.G + g) * (D + 2);
-            const float2 u = *reinterpret_cast<const float2*>(st + c4), w = *reinterpret_cast<const float2*>(st + c4 + 2);
-            s.add(st[D], st[D + 1], make_float4(u.x, u.y, w.x, w.y));
-        }
-    }
-    const bool failed = *reinterpret_cast<volatile int*>(a.c.status) == SA_STATUS_TIMEOUT;
-    const float f = failed ? nanf("") : (s.l > 0.f ? 1.f / s.l : 0.f);
-    const long long at = (long long)b * a.o_stride + (long long)h * D + c4;
-    if constexpr (sizeof(OT) == 4) {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) =
-            make_float4(s.o[0] * f, s.o[1] * f, s.o[2] * f, s.o[3] * f);
-    } else {
-        const __nv_bfloat162 u = __floats2bfloat162_rn(s.o[0] * f, s.o[1] * f);
-        const __nv_bfloat162 w = __floats2bfloat162_rn(s.o[2] * f, s.o[3] * f);
-        uint2 x;
-        x.x = *reinterpret_cast<const uint32_t*>(&u);
-        x.y = *reinterpret_cast<const uint32_t*>(&w);
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = x;
-    }
+    s.store(static_cast<OT*>(a.out) + (long long)b * a.o_stride + (long long)h * D, lane, a.c.status);
 }
 
 struct PrefixWs {
@@ -210,7 +174,7 @@ SA_API int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const
         }
     }
     SA_RC_TRY(pg::decode_launch(ctx, kv, q, q_stride, hq, 0, 0, scale, nullptr, 0, true, ws.own));
-    const long long rows = (long long)kv->n_seqs * hq, per = pg::JT / (d / 4);
+    const long long rows = (long long)kv->n_seqs * hq, per = pg::JT / 32;
     const dim3 grid((unsigned)((rows + per - 1) / per));
     auto k = kv->dtype == SA_F32 ? (d == 64 ? pg::prefix_join_kernel<float, 64> : pg::prefix_join_kernel<float, 128>)
                                  : (d == 64 ? pg::prefix_join_kernel<__nv_bfloat16, 64>

@@ -386,10 +386,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                 float alpha = 1.f, sum;
                 if (c == 0) {
                     m = pf::row_max(sc) * sl2;
-                    sum = pf::emit_p<0, false>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, nullptr);
+                    sum = pf::emit_p2<false>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, nullptr);
                 } else {
                     float mxr;
-                    sum = pf::emit_p<0, true>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, &mxr);
+                    sum = pf::emit_p2<true>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, &mxr);
                     const float mxs = mxr * sl2;
                     const bool need = mxs > m + pf::RESCALE_THRESHOLD;
                     if (__any_sync(0xffffffffu, need)) {
@@ -407,7 +407,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                             tc::tmem_st32(lane_addr + col_o(x) + cb * 32, o);
                         }
                         tc::tmem_wait_st();
-                        sum = pf::emit_p<0, false>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, nullptr);
+                        sum = pf::emit_p2<false>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, nullptr);
                     }
                 }
                 l = l * alpha + sum;
