@@ -128,34 +128,44 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-template <bool TRACK_MAX>
-__device__ __forceinline__ float emit_p2(const float* sc, float sl2, float nm, uint32_t p_addr, float* mx_out) {
-    const unsigned long long s2 = f2(sl2, sl2), n2 = f2(nm, nm);
-    unsigned long long ps[4] = {0ull, 0ull, 0ull, 0ull};
-    float mx[4];
-    if constexpr (TRACK_MAX) {
+// Max of a row's 128 scores, three operands at a time.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float row_max3(const float* sc) {
+    float mx[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i] = sc[i];
+    for (int i = 0; i < 8; ++i) mx[i] = max3(sc[3 * i], sc[3 * i + 1], sc[3 * i + 2]);
+#pragma unroll
+    for (int i = 0; i < 52; ++i) mx[i & 7] = max3(mx[i & 7], sc[24 + 2 * i], sc[25 + 2 * i]);
+    return max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+}
+
+// Bits [0, n) of a word.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+// -infinity where the bit of a row's 32 scores is clear.
+__device__ __forceinline__ void keep_bits(float* sc, uint32_t bits) {
+    if (__all_sync(0xffffffffu, bits == 0xffffffffu)) return;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) sc[i] = (bits & (1u << i)) ? sc[i] : -INFINITY;
+}
+
+// 2^(sc * s2 + n2) of N of a row's scores as N / 2 bf16 pairs in pk, added to
+// the row's sums ps.
+template <int N>
+__device__ __forceinline__ void exp_pairs(const float* sc, unsigned long long s2, unsigned long long n2, uint32_t* pk,
+                                          unsigned long long (&ps)[4]) {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+        float e0, e1;
+        un2(fma2(f2(sc[c], sc[c + 1]), s2, n2), e0, e1);
+        e0 = ex2(e0);
+        e1 = ex2(e1);
+        ps[(c >> 1) & 3] = add2(ps[(c >> 1) & 3], f2(e0, e1));
+        pk[c >> 1] = pack_bf16(e0, e1);
     }
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = hf * 64; c < hf * 64 + 64; c += 2) {
-            if constexpr (TRACK_MAX) mx[(c >> 1) & 3] = fmaxf(fmaxf(mx[(c >> 1) & 3], sc[c]), sc[c + 1]);
-            float e0, e1;
-            un2(fma2(f2(sc[c], sc[c + 1]), s2, n2), e0, e1);
-            e0 = ex2(e0);
-            e1 = ex2(e1);
-            ps[(c >> 1) & 3] = add2(ps[(c >> 1) & 3], f2(e0, e1));
-            pk[(c >> 1) & 31] = pack_bf16(e0, e1);
-        }
-        tc::tmem_st32(p_addr + hf * 32, pk);
-    }
-    if constexpr (TRACK_MAX) *mx_out = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-    float a, b;
-    un2(add2(add2(ps[0], ps[1]), add2(ps[2], ps[3])), a, b);
-    return a + b;
 }
 
 }  // namespace pf

@@ -81,7 +81,7 @@ template <int ST>
 struct TcBars {
     uint64_t q_full;
     uint64_t k_full[ST], k_empty[ST], v_full[ST], v_empty[ST];
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2], p_full[2][2], o_full[2];      // p_full: by slot and half of the keys
     uint64_t drain;
     uint32_t tmem_base;
     int abort;
@@ -186,7 +186,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         }
         for (int x = 0; x < 2; ++x) {
             mbar_init(&B->s_full[x], 1);
-            mbar_init(&B->p_full[x], 4);
+            mbar_init(&B->p_full[x][0], 4);                // one arrival per softmax warp
+            mbar_init(&B->p_full[x][1], 4);
             mbar_init(&B->o_full[x], 1);
         }
         mbar_init(&B->drain, 1);
@@ -256,26 +257,37 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                 for (int j = max(0, v_issued - ST); j < v_issued; ++j)
                     mbar_wait(&B->v_full[j % ST], (j / ST) & 1, nullptr);
             }
-        } else if (warp == 1 && lane == 0 && n_kv > 0) {
+        } else if (warp == 1 && n_kv > 0 && tc::elect_one()) {
             // ---------------------------------------------- MMA issuer
             constexpr uint32_t idS = tc::idesc_bf16_f32(BM, BN, false, false);
             constexpr uint32_t idO = tc::idesc_bf16_f32(BM, D, false, true);
-            const uint32_t sQ = smem_u32(sm + L::Q), sK = smem_u32(sm + L::K), sV = smem_u32(sm + L::V);
+            // descriptors of the first k-step; further ones add to the address field
+            const uint64_t dQ = tc::sdesc_sw128(smem_u32(sm + L::Q), 16, 1024);
+            const uint64_t dK = tc::sdesc_sw128(smem_u32(sm + L::K), 16, 1024);
+            const uint64_t dV = tc::sdesc_sw128(smem_u32(sm + L::V), BOX, 1024);
             auto issue_S = [&](int x, int j) {
-                const uint32_t q = sQ + (alt ? 0 : x) * L::TILE, k = sK + (j % ST) * L::TILE;
+                const uint64_t q = dQ + (uint32_t)((alt ? 0 : x) * (L::TILE >> 4)), k = dK + (uint32_t)((j % ST) * (L::TILE >> 4));
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * BOX + (kk & 3) * 32;
-                    tc::mma_bf16(tbase + col_s(x), tc::sdesc_sw128(q + off, 16, 1024),
-                                 tc::sdesc_sw128(k + off, 16, 1024), idS, kk > 0);
+                    const uint32_t off = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
+                    tc::mma_bf16(tbase + col_s(x), q + off, k + off, idS, kk > 0);
                 }
             };
-            auto issue_PV = [&](int x, int j, bool first) {
-                const uint32_t v = sV + (j % ST) * L::TILE;
+            // P.V of slot x's c-th tile, in two halves of 64 keys as P arrives
+            auto issue_PV = [&](int x, int j, int c) {
+                const uint64_t v = dV + (uint32_t)((j % ST) * (L::TILE >> 4));
 #pragma unroll
-                for (int kk = 0; kk < BN / 16; ++kk)
-                    tc::mma_bf16_ts(tbase + col_o(x), tbase + col_p(x) + kk * 8,
-                                    tc::sdesc_sw128(v + kk * 2048, BOX, 1024), idO, (!first || kk > 0) ? 1u : 0u);
+                for (int half = 0; half < 2; ++half) {
+                    if (!wait_ab(&B->p_full[x][half], c & 1, abort, status)) return false;
+                    tc::fence_after_sync();
+#pragma unroll
+                    for (int k = 0; k < BN / 32; ++k) {
+                        const int kk = half * (BN / 32) + k;
+                        tc::mma_bf16_ts(tbase + col_o(x), tbase + col_p(x) + kk * 8, v + (uint32_t)(kk * 2048 >> 4), idO,
+                                        kk > 0 ? 1u : (uint32_t)(c > 0));
+                    }
+                }
+                return true;
             };
             auto k_ready = [&](int j) { return wait_ab(&B->k_full[j % ST], (j / ST) & 1, abort, status); };
             auto v_ready = [&](int j) { return wait_ab(&B->v_full[j % ST], (j / ST) & 1, abort, status); };
@@ -290,9 +302,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                 }
                 for (int j = 0; ok && j < n_kv; ++j) {
                     const int x = j & 1, c = j >> 1;
-                    if (!(ok = v_ready(j) && wait_ab(&B->p_full[x], c & 1, abort, status))) break;
-                    tc::fence_after_sync();
-                    issue_PV(x, j, c == 0);
+                    if (!(ok = v_ready(j) && issue_PV(x, j, c))) break;
                     tc::mma_commit(&B->v_empty[j % ST]);
                     if (j + 2 >= n_kv) {
                         tc::mma_commit(&B->o_full[x]);
@@ -321,9 +331,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                     for (int x = 0; ok && x < 2; ++x) {
                         const int nx = x ? n1 : n0;
                         if (j >= nx) continue;
-                        if (!(ok = wait_ab(&B->p_full[x], j & 1, abort, status))) break;
-                        tc::fence_after_sync();
-                        issue_PV(x, j, j == 0);
+                        if (!(ok = issue_PV(x, j, j))) break;
                         if (j + 1 == nx) {
                             tc::mma_commit(&B->o_full[x]);
                             continue;
@@ -352,22 +360,28 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
         if (ntok > 0) {
             const int quad = warp & 3, row = quad * 32 + lane;
             const uint32_t lane_addr = tbase + ((uint32_t)(quad * 32) << 16);
+            const uint32_t p_addr = lane_addr + col_p(x);
             const int tok = row / a.G, g = row - tok * a.G;
             const int nx = x ? n1 : n0, p0 = s_unit.p0[x];
             const int len = s_unit.len;
-            // what this row sees: [lo, lo + span) and [0, first)
+            // this row sees [lo, limit] and the first rows; every row of the slot sees
+            // [all_lo, all_hi]
             const int limit = PREFIX ? len - 1 : p0 + tok;
             const int lo = PREFIX ? 0 : window_lo(limit, a.window);
-            const unsigned span = limit < 0 ? 0u : (unsigned)(limit - lo + 1);
-            const int first = PREFIX ? 0 : min(a.sinks, limit + 1);
-            // what every row of the slot sees
             const int all_hi = PREFIX ? len - 1 : p0;
             const int all_lo = PREFIX ? 0 : window_lo(p0 + ntok - 1, a.window);
             const float sl2 = a.sl2;
+            const int j0 = s_unit.j0;
             float m = -INFINITY, l = 0.f;
             bool ok = true;
             for (int c = 0; c < nx; ++c) {
+                // what needs no score is settled before the wait for them
                 const int j = alt ? 2 * c + x : c;
+                const int k0 = t.row0(j0 + j, BN);
+                const bool masked = k0 + BN - 1 > all_hi || !(k0 >= all_lo || k0 + BN <= a.sinks);
+                // the first slot that uses a tile with rows behind the last one clears
+                // them in V: they enter P.V as zeros (the other's P.V is issued later)
+                const bool clear = k0 + BN > len && (alt || x == 0 || j >= n0);
                 if (!(ok = wait_ab(&B->s_full[x], c & 1, abort, status))) break;
                 tc::fence_after_sync();
                 uint32_t u32[BN];
@@ -375,28 +389,22 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                 for (int cb = 0; cb < BN / 32; ++cb) tc::tmem_ld32p(lane_addr + col_s(x) + cb * 32, u32 + cb * 32);
                 tc::tmem_wait_ld();
                 float* sc = reinterpret_cast<float*>(u32);
-                const int k0 = t.row0(s_unit.j0 + j, BN);
-                if (k0 + BN - 1 > all_hi || !(k0 >= all_lo || k0 + BN <= a.sinks)) {
-                    const int rel = k0 - lo;
+                if (masked) {
+                    const int hi = limit + 1 - k0, from = lo - k0, first = PREFIX ? 0 : min(a.sinks, limit + 1) - k0;
 #pragma unroll
-                    for (int i = 0; i < BN; ++i)
-                        if ((unsigned)(rel + i) >= span && k0 + i >= first) sc[i] = -INFINITY;
+                    for (int w = 0; w < 4; ++w)
+                        pf::keep_bits(sc + w * 32, (pf::bits_below(hi - w * 32) & ~pf::bits_below(from - w * 32)) |
+                                                       pf::bits_below(first - w * 32));
                 }
-                const uint32_t p_addr = lane_addr + col_p(x);
-                float alpha = 1.f, sum;
-                if (c == 0) {
-                    m = pf::row_max(sc) * sl2;
-                    sum = pf::emit_p2<false>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, nullptr);
-                } else {
-                    float mxr;
-                    sum = pf::emit_p2<true>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, &mxr);
-                    const float mxs = mxr * sl2;
-                    const bool need = mxs > m + pf::RESCALE_THRESHOLD;
-                    if (__any_sync(0xffffffffu, need)) {
-                        if (need) {
-                            alpha = ex2(m - mxs);
-                            m = mxs;
-                        }
+                // the running maximum moves, and O is rescaled, only when a row's
+                // scores outgrow it by 2^8 (the last P.V completed before S came)
+                const float mxs = pf::row_max3(sc) * sl2;
+                const bool need = mxs > m + pf::RESCALE_THRESHOLD;
+                if (__any_sync(0xffffffffu, need)) {
+                    const float alpha = need ? ex2(m - mxs) : 1.f;
+                    if (need) m = mxs;
+                    l *= alpha;
+                    if (c > 0) {
 #pragma unroll 1
                         for (int cb = 0; cb < D / 32; ++cb) {
                             uint32_t o[32];
@@ -406,14 +414,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
                             tc::tmem_st32(lane_addr + col_o(x) + cb * 32, o);
                         }
-                        tc::tmem_wait_st();
-                        sum = pf::emit_p2<false>(sc, sl2, m == -INFINITY ? 0.f : -m, p_addr, nullptr);
                     }
                 }
-                l = l * alpha + sum;
-                // rows behind the last one enter P.V as zeros; the first slot that
-                // uses the tile clears them (the other's P.V is issued later)
-                if (k0 + BN > len && (alt || x == 0 || j >= n0)) {
+                if (clear) {
                     const int s = j % ST, r0 = max(0, len - k0), n = (BN - r0) * 8 * L::HALVES;
                     if (!(ok = wait_ab(&B->v_full[s], (j / ST) & 1, abort, status))) break;
                     for (int i = row; i < n; i += BM) {
@@ -423,10 +426,29 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                     }
                     fence_proxy_async_smem();
                 }
+                const float nm = m == -INFINITY ? 0.f : -m;
+                const unsigned long long s2 = pf::f2(sl2, sl2), n2 = pf::f2(nm, nm);
+                unsigned long long ps[4] = {0ull, 0ull, 0ull, 0ull};
+                // the first half of P is handed over a quarter of the tile later, when
+                // its stores have long landed; the tensor core needs the time of the
+                // second half for it anyway
+                uint32_t pk[32];
+                pf::exp_pairs<64>(sc, s2, n2, pk, ps);
+                tc::tmem_st32(p_addr, pk);
+                pf::exp_pairs<32>(sc + 64, s2, n2, pk, ps);
                 tc::tmem_wait_st();
                 tc::fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&B->p_full[x]);
+                if (lane == 0) mbar_arrive(&B->p_full[x][0]);
+                pf::exp_pairs<32>(sc + 96, s2, n2, pk + 16, ps);
+                tc::tmem_st32(p_addr + 32, pk);
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&B->p_full[x][1]);
+                float s0, s1;
+                pf::un2(pf::add2(pf::add2(ps[0], ps[1]), pf::add2(ps[2], ps[3])), s0, s1);
+                l += s0 + s1;
             }
             const bool mine = tok < ntok && row < a.tpt * a.G;
             if (ok && (nx == 0 || wait_ab(&B->o_full[x], 0, abort, status))) {
