@@ -128,6 +128,7 @@ struct Joined {
 struct SeqUnit {
     int b, unit;            // sequence, unit of it
     int first, tokens;      // the sequence's first row in the token tensors, its tokens
+    int len;                // its rows
 };
 // Tokens of sequence b; a range outside the token tensors is reported and
 // counts as none.
@@ -148,6 +149,7 @@ __device__ bool find_seq_unit(const Cache& c, const int* cu_q, int n_tok, int pe
     const int run = (c.n_seqs + THREADS - 1) / THREADS;
     const int b0 = min(c.n_seqs, tid * run), b1 = min(c.n_seqs, b0 + run);
     int first, mine = 0;
+    const int len0 = b0 < b1 ? seq_len(c, b0) : 0;       // in flight with cu_q: most runs are one sequence
     for (int b = b0; b < b1; ++b) mine += (seq_tokens(c, cu_q, n_tok, b, &first) + per - 1) / per;
     int inc = mine;
 #pragma unroll
@@ -174,6 +176,7 @@ __device__ bool find_seq_unit(const Cache& c, const int* cu_q, int n_tok, int pe
                 s->unit = want - at;
                 s->first = first;
                 s->tokens = n;
+                s->len = b == b0 ? len0 : seq_len(c, b);
                 break;
             }
             at += u;

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(FT, D == 64 ? 2 : 1) paged_f32_kernel(const __
         const int off = s_seq.unit * a.tpt;
         tok0 = s_seq.first + off;
         ntok = min(a.tpt, s_seq.tokens - off);
-        len = seq_len(a.c, s_seq.b);
+        len = s_seq.len;
         p0 = len - s_seq.tokens + off;
         t = make_unit(p0, max(-1, p0 + ntok - 1), -1, a.window, a.sinks, FN).t;
         j0 = 0;

@@ -25,7 +25,7 @@ struct JoinArgs {
     void* out;
     long long o_stride;
     int hq, G;
-    int n_split, alt_from;       // rows of sequences >= alt_from have 2 n_split parts, the others n_split
+    int parts;
     const float* part_o;
     const float* part_ml;
 };
@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(JT) prefix_join_kernel(const __grid_constant__
     const bool own = seq_len(a.c, b) > 0;
     const int4 rec = own ? a.ws.pair[b * a.c.hkv + kvh] : make_int4(-1, 0, 0, 0);
     Joined<D> s;
-    s.add(b >= a.alt_from ? 2 * a.n_split : a.n_split, lane,
+    s.add(a.parts, lane,
           [&](int p) { return reinterpret_cast<const float2*>(a.part_ml)[p * rows + row]; },
           [&](int p) { return a.part_o + (p * rows + row) * D; });
     if (own && rec.x < 0)
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(JT) prefix_join_kernel(const __grid_constant__
 struct PrefixWs {
     DecodeWs own;
     float *part_o, *part_ml;
-    int n_split;
+    int n_split, parts;
 };
 static size_t prefix_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, int prefix_len, void* base,
                                PrefixWs* ws) {
@@ -66,10 +66,9 @@ static size_t prefix_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq,
     size_t at = align_up(decode_ws_layout(ctx, kv, hq, true, base, &w.own), 256);
     unsigned char* p = static_cast<unsigned char*>(base);
     if (prefix_len > 0) {
-        int parts;
-        if (kv->dtype == SA_F32) parts = w.n_split = f32_prefix_splits(ctx, kv, hq, prefix_len);
-        else w.n_split = tc_prefix_splits(ctx, kv, hq, prefix_len, &parts);
-        const size_t rows = (size_t)parts * kv->n_seqs * hq;
+        if (kv->dtype == SA_F32) w.parts = w.n_split = f32_prefix_splits(ctx, kv, hq, prefix_len);
+        else w.n_split = tc_prefix_splits(ctx, kv, hq, prefix_len, &w.parts);
+        const size_t rows = (size_t)w.parts * kv->n_seqs * hq;
         w.part_o = reinterpret_cast<float*>(p ? p + at : nullptr);
         at += align_up(rows * kv->d * 4, 256);
         w.part_ml = reinterpret_cast<float*>(p ? p + at : nullptr);
@@ -159,10 +158,9 @@ SA_API int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const
     j.o_stride = o_stride;
     j.hq = hq;
     j.G = hq / kv->hkv;
-    j.n_split = ws.n_split;
+    j.parts = ws.parts;
     j.part_o = ws.part_o;
     j.part_ml = ws.part_ml;
-    j.alt_from = kv->n_seqs;
     if (prefix_len > 0) {
         if (kv->dtype == SA_F32) {
             SA_RC_TRY(pg::f32_prefix_launch(ctx, kv, static_cast<const float*>(q), q_stride, hq, prefix_table,
@@ -170,7 +168,6 @@ SA_API int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const
         } else {
             SA_RC_TRY(pg::tc_prefix_launch(ctx, kv, q, q_stride, hq, prefix_table, prefix_len, scale, ws.n_split,
                                            ws.part_o, ws.part_ml));
-            j.alt_from = pg::tc_prefix_alt_from(kv->n_seqs, j.G);
         }
     }
     SA_RC_TRY(pg::decode_launch(ctx, kv, q, q_stride, hq, 0, 0, scale, nullptr, 0, true, ws.own));
