@@ -99,6 +99,16 @@ struct Joined {
             }
         }
     }
+    // Another warp's state (its o in memory, l summed).
+    __device__ __forceinline__ void add_one(int lane, float m2, float l2, const float* row) {
+        const float M = fmaxf(m, m2);
+        if (M == -INFINITY) return;
+        const float wa = ex2(m - M), wb = ex2(m2 - M);
+        m = M;
+        l = l * wa + (lane == 0 ? l2 * wb : 0.f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = o[e] * wa + (wb > 0.f ? row[lane * V + e] * wb : 0.f);
+    }
     __device__ __forceinline__ float total() const {
         float t = l;
 #pragma unroll

@@ -2,15 +2,20 @@
 // the prefill and the shared prefix's part of a decode, as sa_paged_tc.cu does
 // them for bf16.
 //
-// fp32 throughout, on FMAs: the tensor cores take no fp32 operands, and tf32 or
-// bf16 ones would lose what an fp32 cache is kept for.  Bound: FMA issue
-// (4 rows d FLOP per key and head).
+// fp32 results from the tensor cores: an operand x is the sum of two tf32 numbers,
+// hi = x rounded to 11 significant bits and lo = x - hi (exact), and
+//   x y = hi hi' + hi lo' + lo hi'  (+ lo lo', at most 2^-22 of x y, left out),
+// each product exact in the fp32 accumulator; the tensor core drops lo's bits past
+// its eleventh, another 2^-22.  So three mma.m16n8k8 give what an fp32 FMA loop
+// gives to within its own rounding, at 512 / 3 FMA a clock and SM (measured)
+// where FMAs have 128 and spend half of their slots on feeding them.  (bf16
+// pairs would run twice as fast, at 2^-17.)
 //
-// A CTA holds 64 query rows (64 / G tokens times the G heads of a KV head)
-// and walks over tiles of 64 keys: S = Q K^T with a 4 x 4 piece of S per
-// thread, the online softmax on it (a row lies in 16 lanes), P through shared
-// memory, O += P V with 4 rows x D / 16 columns per thread.  K and V of the next
-// tile are copied (cp.async) as soon as their buffers are free: K under the
+// A CTA of eight warps holds FM query rows (FM / G tokens times the G heads of a
+// KV head) and walks over tiles of 64 keys: S = Q K^T with 16 rows per warp, the
+// warps of a row group sharing the keys; the row maximum and P through shared
+// memory; O += P V with the row group's warps sharing O's columns.  K and V of the
+// next tile are copied (cp.async) as soon as their buffers are free: K under the
 // softmax and P V, V under the next S.  Rows that no query of the CTA sees are
 // not read but zero-filled.
 #include <algorithm>
@@ -22,7 +27,7 @@
 namespace sa {
 namespace pg {
 
-constexpr int FM = 64, FN = 64, FT = 256;
+constexpr int FN = 64, FT = 256;
 constexpr float F_LOG2E = 1.4426950408889634f;
 
 struct F32Args {
@@ -38,13 +43,47 @@ struct F32Args {
     float *part_o, *part_ml;
 };
 
-template <int D>
+template <int D, int FM>
 struct FLay {
-    static constexpr int QS = D + 4, PS = FN + 4;      // padded rows: float4 reads of 8 rows hit all banks
-    static constexpr int Q = 0, K = FM * QS, V = K + FN * QS, P = V + FN * D;
-    static constexpr int SMEM = (P + FM * PS) * 4;
+    // Row strides of 4 mod 32 words: the eight rows of an ldmatrix, and the V
+    // elements of a fragment (rows two apart, eight columns), hit all banks.
+    static constexpr int RS = D + 4, PS = FN + 4;
+    static constexpr int WM = FM / 16, WN = 8 / WM;    // warps over rows; over keys, then over columns
+    static constexpr int Q = 0, K = FM * RS, V = K + FN * RS, P = V + FN * RS, X = P + FM * PS;
+    static constexpr int SMEM = (X + WN * FM) * 4;
 };
 
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
+    hi = (x + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+}
+__device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// c += A B of one step: the tensor core cuts its sums off where fp32 rounds, so
+// it sums eight products from zero and the long sum is an fp32 addition.
+__device__ __forceinline__ void mma_exact(float (&c)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t bh0,
+                                          uint32_t bh1, uint32_t bl0, uint32_t bl1) {
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+    mma1688(d, al, bh0, bh1);
+    mma1688(d, ah, bl0, bl1);
+    mma1688(d, ah, bh0, bh1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] += d[e];
+}
+// 8x4 blocks of 32-bit words: lane's word is (lane / 4, lane % 4) of each block,
+// lane l gives the address of row l % 8 of block l / 8.
+__device__ __forceinline__ void ldsm4w(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t r;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(addr) : "memory");
+    return r;
+}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
@@ -52,15 +91,18 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <int D, bool PREFIX>
-__global__ void __launch_bounds__(FT, D == 64 ? 2 : 1) paged_f32_kernel(const __grid_constant__ F32Args a) {
-    using L = FLay<D>;
-    constexpr int CC = D / 64;                           // float4 columns per thread
+template <int D, int FM, bool PREFIX>
+__global__ void __launch_bounds__(FT, (FM == 32 || D == 64) ? 2 : 1) paged_f32_kernel(const __grid_constant__ F32Args a) {
+    using L = FLay<D, FM>;
+    constexpr int NT = FN / L::WN / 8;                   // 8-key blocks of S per warp
+    constexpr int CT = D / L::WN / 8;                    // 8-column blocks of O per warp
     extern __shared__ __align__(16) float smf[];
     __shared__ SeqUnit s_seq;
     __shared__ int s_scan[FT / 32];
-    float *sQ = smf + L::Q, *sK = smf + L::K, *sV = smf + L::V, *sP = smf + L::P;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    float *sQ = smf + L::Q, *sK = smf + L::K, *sV = smf + L::V, *sP = smf + L::P, *sX = smf + L::X;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int wm = warp % L::WM, wn = warp / L::WM;      // the warp's 16 rows; its keys and columns
+    const int fr = lane >> 2, fc = lane & 3;             // row and word of a fragment
     if (PREFIX) pdl_trigger();
 
     int kvh, tok0, ntok, p0, len, j0, n_kv, split = 0;
@@ -93,19 +135,9 @@ __global__ void __launch_bounds__(FT, D == 64 ? 2 : 1) paged_f32_kernel(const __
         row_table = a.c.table + (long long)s_seq.b * a.c.table_stride;
     }
 
-    // ---- Q, scaled (into exponents of two) on the way
-    for (int i = tid; i < FM * (D / 4); i += FT) {
-        const int r = i / (D / 4), c4 = i - r * (D / 4), tk = r / a.G, g = r - tk * a.G;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (tk < ntok)
-            x = *reinterpret_cast<const float4*>(a.q + (long long)(tok0 + tk) * a.q_tok + (long long)(kvh * a.G + g) * D +
-                                                 c4 * 4);
-        x.x *= a.qscale; x.y *= a.qscale; x.z *= a.qscale; x.w *= a.qscale;
-        *reinterpret_cast<float4*>(sQ + r * L::QS + c4 * 4) = x;
-    }
     // ---- copies: four threads per key row
     const int cr = tid >> 2, cq = tid & 3;
-    const uint32_t kdst = smem_u32(sK + cr * L::QS + cq * 4), vdst = smem_u32(sV + cr * D + cq * 4);
+    const uint32_t kdst = smem_u32(sK + cr * L::RS + cq * 4), vdst = smem_u32(sV + cr * L::RS + cq * 4);
     auto place = [&](int j) -> long long {               // this thread's row of tile j in the pools, -1: zeros
         const int row = t.row0(j0 + j, FN) + cr;
         if (j >= n_kv || !t.sees(row)) return -1;
@@ -126,144 +158,189 @@ __global__ void __launch_bounds__(FT, D == 64 ? 2 : 1) paged_f32_kernel(const __
         copy(vdst, a.c.v, at);
     }
 
-    // what this thread's rows see
-    int lo[4], first[4];
-    unsigned span[4];
+    // ---- Q, scaled (into exponents of two) on the way
+    constexpr int QL = FM * (D / 4) / FT;                // float4 per thread
+    float4 qv[QL];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int limit = PREFIX ? len - 1 : p0 + (ty * 4 + i) / a.G;
+    for (int u = 0; u < QL; ++u) {
+        const int i = tid + u * FT, r = i / (D / 4), c4 = i - r * (D / 4), tk = r / a.G, g = r - tk * a.G;
+        qv[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (tk < ntok)
+            qv[u] = *reinterpret_cast<const float4*>(a.q + (long long)(tok0 + tk) * a.q_tok +
+                                                     (long long)(kvh * a.G + g) * D + c4 * 4);
+    }
+#pragma unroll
+    for (int u = 0; u < QL; ++u) {
+        const int i = tid + u * FT, r = i / (D / 4), c4 = i - r * (D / 4);
+        *reinterpret_cast<float4*>(sQ + r * L::RS + c4 * 4) =
+            make_float4(qv[u].x * a.qscale, qv[u].y * a.qscale, qv[u].z * a.qscale, qv[u].w * a.qscale);
+    }
+
+    // what this lane's rows (fr and fr + 8 of the warp's) see
+    int lo[2], first[2];
+    unsigned span[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int limit = PREFIX ? len - 1 : p0 + (wm * 16 + fr + 8 * i) / a.G;
         lo[i] = PREFIX ? 0 : window_lo(limit, a.window);
         span[i] = limit < 0 ? 0u : (unsigned)(limit - lo[i] + 1);
         first[i] = PREFIX ? 0 : min(a.sinks, limit + 1);
     }
     const int all_lo = PREFIX ? 0 : window_lo(p0 + ntok - 1, a.window);
-    float m[4], l[4], o[4][CC][4];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[CT][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        m[i] = -INFINITY;
-        l[i] = 0.f;
+    for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int c = 0; c < CC; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][c][e] = 0.f;
-    }
+        for (int e = 0; e < 4; ++e) o[c][e] = 0.f;
+    // ldmatrix addresses: A (16 rows x 8 words): blocks by rows, then words; B (two
+    // 8-key blocks x 8 words): blocks by words, then keys
+    const int ar = wm * 16 + (lane & 15), aw = (lane >> 4) * 4;
+    const uint32_t qa = smem_u32(sQ + ar * L::RS + aw), pa = smem_u32(sP + ar * L::PS + aw);
+    const uint32_t kb = smem_u32(sK + (wn * NT * 8 + (lane >> 4) * 8 + (lane & 7)) * L::RS + ((lane >> 3) & 1) * 4);
+    // V: the eight keys of a step enter in the order that P's accumulator has them
+    const uint32_t vb = smem_u32(sV + 2 * fc * L::RS + wn * CT * 8 + fr);
 
     for (int j = 0; j < n_kv; ++j) {
         const long long next = place(j + 1);
         cp_wait<1>();                                    // K of this tile (V is the group after it)
         __syncthreads();
-        float s[4][4];
+        float s[NT][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[i][k] = 0.f;
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll 4
-        for (int c = 0; c < D; c += 4) {
-            float4 qv[4], kv[4];
+        for (int k = 0; k < D; k += 8) {
+            uint32_t x[4], ah[4], al[4];
+            ldsm4w(x, qa + k * 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) qv[i] = *reinterpret_cast<const float4*>(sQ + (ty * 4 + i) * L::QS + c);
+            for (int e = 0; e < 4; ++e) split_tf32(x[e], ah[e], al[e]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) kv[k] = *reinterpret_cast<const float4*>(sK + (tx + 16 * k) * L::QS + c);
+            for (int n = 0; n < NT; n += 2) {
+                uint32_t y[4], bh[4], bl[4];
+                ldsm4w(y, kb + (n * 8 * L::RS + k) * 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int e = 0; e < 4; ++e) split_tf32(y[e], bh[e], bl[e]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    s[i][k] = fmaf(qv[i].x, kv[k].x, s[i][k]);
-                    s[i][k] = fmaf(qv[i].y, kv[k].y, s[i][k]);
-                    s[i][k] = fmaf(qv[i].z, kv[k].z, s[i][k]);
-                    s[i][k] = fmaf(qv[i].w, kv[k].w, s[i][k]);
+                for (int h = 0; h < 2; ++h) {
+                    mma_exact(s[n + h], ah, al, bh[2 * h], bh[2 * h + 1], bl[2 * h], bl[2 * h + 1]);
                 }
+            }
         }
+        // accumulator: rows fr, fr + 8; keys 2 fc, 2 fc + 1 of each block
         const int k0 = t.row0(j0 + j, FN);
         if (k0 + FN - 1 > p0 || !(k0 >= all_lo || k0 + FN <= a.sinks)) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int key = k0 + tx + 16 * k;
-                    if ((unsigned)(key - lo[i]) >= span[i] && key >= first[i]) s[i][k] = -INFINITY;
+                for (int e = 0; e < 4; ++e) {
+                    const int key = k0 + (wn * NT + n) * 8 + 2 * fc + (e & 1), i = e >> 1;
+                    if ((unsigned)(key - lo[i]) >= span[i] && key >= first[i]) s[n][e] = -INFINITY;
                 }
         }
+        float mx[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+        for (int i = 0; i < 2; ++i) {
+            mx[i] = fmaxf(s[0][2 * i], s[0][2 * i + 1]);
 #pragma unroll
-            for (int off = 1; off < 16; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            const float M = fmaxf(m[i], mx), z = M == -INFINITY ? 0.f : M;
+            for (int n = 1; n < NT; ++n) mx[i] = fmaxf(mx[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]));
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+            mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+            if (fc == 0) sX[wn * FM + wm * 16 + fr + 8 * i] = mx[i];
+        }
+        __syncthreads();                                 // the other warps' maxima; everyone is done with K
+        if (j + 1 < n_kv) copy(kdst, a.c.k, next);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int w = 0; w < L::WN; ++w) mx[i] = fmaxf(mx[i], sX[w * FM + wm * 16 + fr + 8 * i]);
+            const float M = fmaxf(m[i], mx[i]), z = M == -INFINITY ? 0.f : M;
             const float corr = ex2(m[i] - z);            // m = -inf: 0
+            m[i] = M;
             float ps = 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float p = ex2(s[i][k] - z);
-                ps += p;
-                sP[(ty * 4 + i) * L::PS + tx + 16 * k] = p;
+            for (int n = 0; n < NT; ++n) {
+                const float p0_ = ex2(s[n][2 * i] - z), p1_ = ex2(s[n][2 * i + 1] - z);
+                ps += p0_ + p1_;
+                // key 2 fc goes to word fc of the step, key 2 fc + 1 to word fc + 4
+                float* dst = sP + (wm * 16 + fr + 8 * i) * L::PS + (wn * NT + n) * 8 + fc;
+                dst[0] = p0_;
+                dst[4] = p1_;
             }
-            l[i] = l[i] * corr + ps;                     // this lane's keys; the 16 lanes are added at the end
-            m[i] = M;
+            l[i] = l[i] * corr + ps;                     // this lane's keys; added up at the end
 #pragma unroll
-            for (int c = 0; c < CC; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][c][e] *= corr;
+            for (int c = 0; c < CT; ++c) {
+                o[c][2 * i] *= corr;
+                o[c][2 * i + 1] *= corr;
+            }
         }
-        cp_wait<0>();                                    // V of this tile
-        __syncthreads();                                 // and everyone is done with K, and P is there
-        if (j + 1 < n_kv) copy(kdst, a.c.k, next);
+        if (j + 1 < n_kv) cp_wait<1>();                  // V of this tile (K of the next came after it)
+        else cp_wait<0>();
+        __syncthreads();                                 // P and V are there
 #pragma unroll 4
-        for (int k = 0; k < FN; k += 4) {
-            float4 pv[4];
+        for (int k = 0; k < FN; k += 8) {
+            uint32_t x[4], ah[4], al[4];
+            ldsm4w(x, pa + k * 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pv[i] = *reinterpret_cast<const float4*>(sP + (ty * 4 + i) * L::PS + k);
+            for (int e = 0; e < 4; ++e) split_tf32(x[e], ah[e], al[e]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int c = 0; c < CT; ++c) {
+                uint32_t bh[2], bl[2];
 #pragma unroll
-                for (int c = 0; c < CC; ++c) {
-                    const float4 v = *reinterpret_cast<const float4*>(sV + (k + e) * D + c * 64 + tx * 4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = e == 0 ? pv[i].x : e == 1 ? pv[i].y : e == 2 ? pv[i].z : pv[i].w;
-                        o[i][c][0] = fmaf(p, v.x, o[i][c][0]);
-                        o[i][c][1] = fmaf(p, v.y, o[i][c][1]);
-                        o[i][c][2] = fmaf(p, v.z, o[i][c][2]);
-                        o[i][c][3] = fmaf(p, v.w, o[i][c][3]);
-                    }
-                }
+                for (int e = 0; e < 2; ++e) split_tf32(lds32(vb + ((k + e) * L::RS + c * 8) * 4), bh[e], bl[e]);
+                mma_exact(o[c], ah, al, bh[0], bh[1], bl[0], bl[1]);
+            }
         }
         __syncthreads();                                 // V and P are free
         if (j + 1 < n_kv) copy(vdst, a.c.v, next);
     }
 
+    // a row's sum: over its four lanes, then over the row group's warps
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if (fc == 0) sX[wn * FM + wm * 16 + fr + 8 * i] = l[i];
+    }
+    __syncthreads();
 #pragma unroll
-        for (int off = 1; off < 16; off <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
-        const int r = ty * 4 + i, tk = r / a.G, g = r - tk * a.G;
+    for (int i = 0; i < 2; ++i) {
+        const int r = wm * 16 + fr + 8 * i, tk = r / a.G, g = r - tk * a.G;
         if (tk >= ntok) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < L::WN; ++w) sum += sX[w * FM + r];
         const int h = kvh * a.G + g;
         float* dst;
         float f = 1.f;
         if constexpr (PREFIX) {
             const long long row = ((long long)split * a.n_tok + tok0 + tk) * a.hq + h;
-            if (tx == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m[i], l[i]);
+            if (wn == 0 && fc == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m[i], sum);
             dst = a.part_o + row * D;
         } else {
             dst = a.out + (long long)(tok0 + tk) * a.o_tok + (long long)h * D;
-            f = l[i] > 0.f ? 1.f / l[i] : 0.f;
+            f = sum > 0.f ? 1.f / sum : 0.f;
         }
 #pragma unroll
-        for (int c = 0; c < CC; ++c)
-            *reinterpret_cast<float4*>(dst + c * 64 + tx * 4) =
-                make_float4(o[i][c][0] * f, o[i][c][1] * f, o[i][c][2] * f, o[i][c][3] * f);
+        for (int c = 0; c < CT; ++c)
+            *reinterpret_cast<float2*>(dst + (wn * CT + c) * 8 + 2 * fc) = make_float2(o[c][2 * i] * f, o[c][2 * i + 1] * f);
     }
 }
 
-template <int D, bool PREFIX>
-static int f32_launch_d(cudaStream_t st, long long grid, const F32Args& a) {
+template <int D, int FM, bool PREFIX>
+static int f32_launch_k(cudaStream_t st, long long grid, const F32Args& a) {
     SA_CHECK_ARG(grid < (1LL << 31), "fp32 attention: %lld CTAs", grid);
-    auto k = paged_f32_kernel<D, PREFIX>;
-    SA_RC_TRY(set_smem_attr_once((const void*)k, FLay<D>::SMEM));
-    k<<<(unsigned)grid, FT, FLay<D>::SMEM, st>>>(a);
+    auto k = paged_f32_kernel<D, FM, PREFIX>;
+    SA_RC_TRY(set_smem_attr_once((const void*)k, FLay<D, FM>::SMEM));
+    k<<<(unsigned)grid, FT, FLay<D, FM>::SMEM, st>>>(a);
     SA_CUDA_TRY(cudaGetLastError());
     return SA_OK;
+}
+template <bool PREFIX>
+static int f32_launch(int d, int fm, cudaStream_t st, long long grid, const F32Args& a) {
+    if (d == 64)
+        return fm == 32 ? f32_launch_k<64, 32, PREFIX>(st, grid, a) : f32_launch_k<64, 64, PREFIX>(st, grid, a);
+    return fm == 32 ? f32_launch_k<128, 32, PREFIX>(st, grid, a) : f32_launch_k<128, 64, PREFIX>(st, grid, a);
 }
 
 int f32_prefill_launch(sa_ctx* ctx, const sa_paged_kv* kv, const float* q, long long q_tok, int n_tok, int hq,
@@ -271,19 +348,25 @@ int f32_prefill_launch(sa_ctx* ctx, const sa_paged_kv* kv, const float* q, long 
     F32Args a = {};
     a.c = make_cache(ctx, kv);
     a.q = q; a.cu_q = cu_q; a.q_tok = q_tok; a.o_tok = o_tok;
-    a.n_tok = n_tok; a.hq = hq; a.G = hq / kv->hkv; a.tpt = FM / a.G;
+    a.n_tok = n_tok; a.hq = hq; a.G = hq / kv->hkv;
     a.window = window; a.sinks = sinks;
     a.qscale = scale * F_LOG2E;
     a.out = out;
-    const long long units = (long long)n_tok / a.tpt + std::min(kv->n_seqs, n_tok);
-    return kv->d == 64 ? f32_launch_d<64, false>(ctx->stream, units * kv->hkv, a)
-                       : f32_launch_d<128, false>(ctx->stream, units * kv->hkv, a);
+    // 64 rows read K and V half as often as 32; 32 where 64 would leave SMs idle
+    const int seqs = std::min(kv->n_seqs, n_tok);
+    auto units = [&](int fm) { return ((long long)n_tok / (fm / a.G) + seqs) * kv->hkv; };
+    const int fm = units(64) < 2 * ctx->num_sms ? 32 : 64;
+    a.tpt = fm / a.G;
+    return f32_launch<false>(kv->d, fm, ctx->stream, units(fm), a);
 }
 
+// Rows of a CTA behind a shared prefix: 32 where they hold all rows of a KV head.
+static int f32_prefix_rows(const sa_paged_kv* kv, int G) { return kv->n_seqs <= 32 / G ? 32 : 64; }
+
 int f32_prefix_splits(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, int prefix_len) {
-    const int tpt = FM / (hq / kv->hkv), units = (kv->n_seqs + tpt - 1) / tpt;
+    const int G = hq / kv->hkv, fm = f32_prefix_rows(kv, G), tpt = fm / G, units = (kv->n_seqs + tpt - 1) / tpt;
     const int tiles = (int)(((long long)prefix_len + FN - 1) / FN);
-    const int slots = ctx->num_sms * (kv->d == 64 ? 2 : 1);
+    const int slots = ctx->num_sms * ((kv->d == 64 || fm == 32) ? 2 : 1);
     return std::max(1, std::min(tiles, slots / std::max(1, units * kv->hkv)));
 }
 
@@ -292,14 +375,15 @@ int f32_prefix_launch(sa_ctx* ctx, const sa_paged_kv* kv, const float* q, long l
     F32Args a = {};
     a.c = make_cache(ctx, kv);
     a.q = q; a.q_tok = q_tok;
-    a.n_tok = kv->n_seqs; a.hq = hq; a.G = hq / kv->hkv; a.tpt = FM / a.G;
+    a.n_tok = kv->n_seqs; a.hq = hq; a.G = hq / kv->hkv;
+    const int fm = f32_prefix_rows(kv, a.G);
+    a.tpt = fm / a.G;
     a.qscale = scale * F_LOG2E;
     a.prefix_table = prefix_table; a.prefix_len = prefix_len;
     a.n_split = n_split;
     a.units = (kv->n_seqs + a.tpt - 1) / a.tpt;
     a.part_o = part_o; a.part_ml = part_ml;
-    const long long grid = (long long)a.units * kv->hkv * n_split;
-    return kv->d == 64 ? f32_launch_d<64, true>(ctx->stream, grid, a) : f32_launch_d<128, true>(ctx->stream, grid, a);
+    return f32_launch<true>(kv->d, fm, ctx->stream, (long long)a.units * kv->hkv * n_split, a);
 }
 
 }  // namespace pg

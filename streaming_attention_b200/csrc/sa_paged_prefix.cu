@@ -17,7 +17,7 @@
 namespace sa {
 namespace pg {
 
-constexpr int JT = 256;
+constexpr int JT = 128;
 
 struct JoinArgs {
     Cache c;
@@ -30,28 +30,41 @@ struct JoinArgs {
     const float* part_ml;
 };
 
-// A warp per (sequence, query head).
+// Four warps per (sequence, query head): a quarter of the prefix's parts each,
+// the last one the sequence's own rows too.
 template <typename OT, int D>
 __global__ void __launch_bounds__(JT) prefix_join_kernel(const __grid_constant__ JoinArgs a) {
+    constexpr int W = JT / 32, V = D / 32;
+    __shared__ float s_o[W - 1][D];
+    __shared__ float2 s_ml[W - 1];
     pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * (JT / 32) + (threadIdx.x >> 5);
-    const long long rows = (long long)a.c.n_seqs * a.hq;
-    if (row >= rows) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long row = blockIdx.x, rows = (long long)a.c.n_seqs * a.hq;
     const int b = (int)(row / a.hq), h = (int)(row - (long long)b * a.hq), kvh = h / a.G, g = h - kvh * a.G;
-    const bool own = seq_len(a.c, b) > 0;
-    const int4 rec = own ? a.ws.pair[b * a.c.hkv + kvh] : make_int4(-1, 0, 0, 0);
+    const int p0 = warp * a.parts / W, p1 = (warp + 1) * a.parts / W;
     Joined<D> s;
-    s.add(a.parts, lane,
-          [&](int p) { return reinterpret_cast<const float2*>(a.part_ml)[p * rows + row]; },
-          [&](int p) { return a.part_o + (p * rows + row) * D; });
-    if (own && rec.x < 0)
-        s.add(1, lane, [&](int) { return a.ws.state_ml[row]; }, [&](int) { return a.ws.state_o + row * D; });
-    if (own && rec.x >= 0) {
-        auto at = [&](int p) { return (2LL * (rec.x + p) + (p == 0 ? rec.z : 0)) * a.G + g; };
-        s.add(rec.y - rec.x + 1, lane, [&](int p) { return a.ws.slot_ml[at(p)]; },
-              [&](int p) { return a.ws.slot_o + at(p) * D; });
+    s.add(p1 - p0, lane, [&](int p) { return reinterpret_cast<const float2*>(a.part_ml)[(p0 + p) * rows + row]; },
+          [&](int p) { return a.part_o + ((p0 + p) * rows + row) * D; });
+    if (warp == W - 1 && seq_len(a.c, b) > 0) {
+        const int4 rec = a.ws.pair[b * a.c.hkv + kvh];
+        if (rec.x < 0) {
+            s.add(1, lane, [&](int) { return a.ws.state_ml[row]; }, [&](int) { return a.ws.state_o + row * D; });
+        } else {
+            auto at = [&](int p) { return (2LL * (rec.x + p) + (p == 0 ? rec.z : 0)) * a.G + g; };
+            s.add(rec.y - rec.x + 1, lane, [&](int p) { return a.ws.slot_ml[at(p)]; },
+                  [&](int p) { return a.ws.slot_o + at(p) * D; });
+        }
     }
+    if (warp > 0) {
+        const float l = s.total();
+        if (lane == 0) s_ml[warp - 1] = make_float2(s.m, l);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s_o[warp - 1][lane * V + e] = s.o[e];
+    }
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 0; w < W - 1; ++w) s.add_one(lane, s_ml[w].x, s_ml[w].y, s_o[w]);
     s.store(static_cast<OT*>(a.out) + (long long)b * a.o_stride + (long long)h * D, lane, a.c.status);
 }
 
@@ -171,8 +184,7 @@ SA_API int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const
         }
     }
     SA_RC_TRY(pg::decode_launch(ctx, kv, q, q_stride, hq, 0, 0, scale, nullptr, 0, true, ws.own));
-    const long long rows = (long long)kv->n_seqs * hq, per = pg::JT / 32;
-    const dim3 grid((unsigned)((rows + per - 1) / per));
+    const dim3 grid((unsigned)(kv->n_seqs * (long long)hq));
     auto k = kv->dtype == SA_F32 ? (d == 64 ? pg::prefix_join_kernel<float, 64> : pg::prefix_join_kernel<float, 128>)
                                  : (d == 64 ? pg::prefix_join_kernel<__nv_bfloat16, 64>
                                             : pg::prefix_join_kernel<__nv_bfloat16, 128>);
