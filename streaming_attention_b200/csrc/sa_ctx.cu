@@ -57,11 +57,12 @@ int ensure_stage(sa_ctx* ctx, size_t bytes) {
 
 int sync_and_check(sa_ctx* ctx) {
     SA_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
-    int st = 0;
-    SA_CUDA_TRY(cudaMemcpy(&st, ctx->status, sizeof(int), cudaMemcpyDeviceToHost));
+    int words[2] = {0, 0};
+    SA_CUDA_TRY(cudaMemcpy(words, ctx->status, sizeof(words), cudaMemcpyDeviceToHost));
+    const int st = words[0] != SA_STATUS_OK ? words[0] : words[1];
     if (st != SA_STATUS_OK) {
-        int zero = 0;
-        cudaMemcpy(ctx->status, &zero, sizeof(int), cudaMemcpyHostToDevice);
+        const int zero[2] = {0, 0};
+        cudaMemcpy(ctx->status, zero, sizeof(zero), cudaMemcpyHostToDevice);
         if (st == SA_STATUS_TIMEOUT)
             return set_error(SA_ERR_TIMEOUT, "a device-side wait exceeded its limit");
         return set_error(SA_ERR_RANGE, "a kernel reported an out-of-range index (status %d)", st);
@@ -106,7 +107,7 @@ SA_API int sa_ctx_create(int device, sa_ctx** out) {
     c->num_sms = prop.multiProcessorCount;
     if (cudaStreamCreateWithFlags(&c->own_stream, cudaStreamNonBlocking) != cudaSuccess ||
         cudaMalloc(&c->counters, SA_MAX_KV_HEADS * sizeof(unsigned)) != cudaSuccess ||
-        cudaMalloc(&c->status, sizeof(int)) != cudaSuccess) {
+        cudaMalloc(&c->status, 2 * sizeof(int)) != cudaSuccess) {
         cudaError_t e = cudaGetLastError();
         if (c->counters) cudaFree(c->counters);
         if (c->own_stream) cudaStreamDestroy(c->own_stream);
@@ -115,7 +116,7 @@ SA_API int sa_ctx_create(int device, sa_ctx** out) {
     }
     c->stream = c->own_stream;
     SA_CUDA_TRY(cudaMemset(c->counters, 0, SA_MAX_KV_HEADS * sizeof(unsigned)));
-    SA_CUDA_TRY(cudaMemset(c->status, 0, sizeof(int)));
+    SA_CUDA_TRY(cudaMemset(c->status, 0, 2 * sizeof(int)));
     *out = c;
     return SA_OK;
 }

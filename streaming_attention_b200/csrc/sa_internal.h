@@ -27,7 +27,10 @@ struct sa_ctx {
     // per-KV-head arrival counters for the decode kernel's last-CTA merge;
     // zero between launches (the last CTA resets its counter)
     unsigned* counters = nullptr;
-    // device status word: 0 ok, else a SA_STATUS_* code set by a kernel
+    // device status words: 0 ok, else a SA_STATUS_* code set by a kernel.  The
+    // second one is for rows and pages that the paged operators were given wrongly:
+    // those calls leave the bad rows out and go on, and no later call is to fail
+    // for it, as kernels do that find the first one set.
     int* status = nullptr;
     // grow-only device staging for SA_HOST_PTRS calls
     void* stage = nullptr;

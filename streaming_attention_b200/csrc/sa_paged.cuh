@@ -25,14 +25,15 @@ struct Cache {
     long long page_stride;     // elements between pages
     long long table_stride;
     int n_pages, page_log2, hkv, n_seqs, max_pages;
-    int* status;
+    int* status;               // expired waits
+    int* bad;                  // rows and pages outside the cache
 };
 
 // Rows of sequence b, within [0, max_pages * page]; a length past what the
 // block table can hold is reported and cut.
 __device__ __forceinline__ int seq_len(const Cache& c, int b) {
     const int n = c.kv_lens[b], cut = cut_len(n, c.max_pages, c.page_log2);
-    if (cut < n) atomicExch(c.status, SA_STATUS_BAD_INDEX);
+    if (cut < n) atomicExch(c.bad, SA_STATUS_BAD_INDEX);
     return cut;
 }
 
@@ -40,7 +41,7 @@ __device__ __forceinline__ int seq_len(const Cache& c, int b) {
 // the pool's.
 __device__ __forceinline__ int checked_page(const Cache& c, int entry) {
     if (page_ok(entry, c.n_pages)) return entry;
-    atomicExch(c.status, SA_STATUS_BAD_INDEX);
+    atomicExch(c.bad, SA_STATUS_BAD_INDEX);
     return -1;
 }
 
@@ -140,16 +141,12 @@ struct SeqUnit {
     int first, tokens;      // the sequence's first row in the token tensors, its tokens
     int len;                // its rows
 };
-// Tokens of sequence b; a range outside the token tensors is reported and
-// counts as none.
-__device__ __forceinline__ int seq_tokens(const Cache& c, const int* cu_q, int n_tok, int b, int* first) {
-    const int c0 = cu_q[b], c1 = cu_q[b + 1];
-    *first = c0;
-    if (c0 < 0 || c1 > n_tok || c1 < c0) {
-        atomicExch(c.status, SA_STATUS_BAD_INDEX);
-        return 0;
-    }
-    return c1 - c0;
+// Tokens of a sequence; a range outside the token tensors is reported and counts
+// as none.
+__device__ __forceinline__ int seq_tokens(const Cache& c, int c0, int c1, int n_tok) {
+    if (c0 >= 0 && c1 <= n_tok && c1 >= c0) return c1 - c0;
+    atomicExch(c.bad, SA_STATUS_BAD_INDEX);
+    return 0;
 }
 // Unit total - 1 - back of the batch, by the whole block (scan: THREADS / 32
 // ints); false when there is none.
@@ -158,9 +155,16 @@ __device__ bool find_seq_unit(const Cache& c, const int* cu_q, int n_tok, int pe
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int run = (c.n_seqs + THREADS - 1) / THREADS;
     const int b0 = min(c.n_seqs, tid * run), b1 = min(c.n_seqs, b0 + run);
-    int first, mine = 0;
+    int mine = 0;
     const int len0 = b0 < b1 ? seq_len(c, b0) : 0;       // in flight with cu_q: most runs are one sequence
-    for (int b = b0; b < b1; ++b) mine += (seq_tokens(c, cu_q, n_tok, b, &first) + per - 1) / per;
+    for (int b = b0; b < b1; b += 8) {                   // eight loads in flight where runs are long
+        int cu[9];
+#pragma unroll
+        for (int u = 0; u < 9; ++u) cu[u] = cu_q[min(b + u, b1)];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (b + u < b1) mine += (seq_tokens(c, cu[u], cu[u + 1], n_tok) + per - 1) / per;
+    }
     int inc = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -180,7 +184,7 @@ __device__ bool find_seq_unit(const Cache& c, const int* cu_q, int n_tok, int pe
     int at = before + inc - mine;
     if (want >= at && want < at + mine)
         for (int b = b0; b < b1; ++b) {
-            const int n = seq_tokens(c, cu_q, n_tok, b, &first), u = (n + per - 1) / per;
+            const int first = cu_q[b], n = seq_tokens(c, first, cu_q[b + 1], n_tok), u = (n + per - 1) / per;
             if (want < at + u) {
                 s->b = b;
                 s->unit = want - at;
@@ -264,6 +268,7 @@ inline Cache make_cache(const sa_ctx* ctx, const sa_paged_kv* kv) {
     c.n_seqs = kv->n_seqs;
     c.max_pages = kv->max_pages;
     c.status = ctx->status;
+    c.bad = ctx->status + 1;
     return c;
 }
 

@@ -118,7 +118,7 @@ __device__ __forceinline__ Place find_place(const AppendArgs& a, int tok, int la
     }
     const long long at = append_row(len, n, t, a.c.max_pages, a.c.page_log2, a.pos0, a.cos_t ? a.n_pos : 1LL << 40);
     if (at < 0) {
-        if (lane == 0) atomicExch(a.c.status, SA_STATUS_BAD_INDEX);
+        if (lane == 0) atomicExch(a.c.bad, SA_STATUS_BAD_INDEX);
         return p;
     }
     p.pos = (int)(a.pos0 + at);

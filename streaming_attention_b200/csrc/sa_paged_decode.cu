@@ -97,7 +97,14 @@ __device__ void plan_share(const DecodeArgs& a, int tk, Share* s, long long* sca
     const int per = (a.c.n_seqs + THREADS - 1) / THREADS;
     const int b0 = tid * per, b1 = min(a.c.n_seqs, b0 + per);
     long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += make_tiles(seq_len(a.c, b), a.window, a.sinks, tk).n;
+    for (int b = b0; b < b1; b += 8) {                   // eight loads in flight where runs are long
+        int len[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) len[u] = b + u < b1 ? a.c.kv_lens[b + u] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            mine += make_tiles(cut_len(len[u], a.c.max_pages, a.c.page_log2), a.window, a.sinks, tk).n;
+    }
     mine *= a.c.hkv;
     long long inc = mine;
 #pragma unroll
@@ -292,7 +299,7 @@ __device__ __forceinline__ void drain(Ring* r) {
 // (neither reads what the other writes); it ends only after that kernel, so that
 // the join, which waits for this one, has both.
 __device__ __forceinline__ void leave(const DecodeArgs& a) {
-    if (a.to_state) pdl_wait();
+    if (a.to_state) pdl_wait();                          // (nothing to wait for in an ordinary launch)
 }
 
 // ---- bf16 -------------------------------------------------------------------
@@ -343,7 +350,6 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     constexpr int TK = Z::TK, KB = TK / 16 / BW;       // blocks of 16 rows per warp and tile
     extern __shared__ unsigned char smem_raw[];
     __shared__ Ring r;
-    __shared__ Dest s_dest;
     const uint32_t raw = smem_u32(smem_raw);
     unsigned char* buf = smem_raw + (((raw + 1023u) & ~1023u) - raw);
     float* red = reinterpret_cast<float*>(buf + STAGES * Z::STAGE_BYTES);
@@ -378,15 +384,9 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     }
     const int qc = lane >> 2, qp = (lane & 3) * 2;      // column as operand; first of two columns as accumulator
     const uint32_t sbuf = smem_u32(buf);
-    int it = 0;
-    bool ok = true;
-    while (ok && w.left > 0) {
-        // ---- one pair's tiles
-        const int b = w.b, h = w.h, i0 = w.i;
-        const Tiles t = w.t;
-        const int i1 = min(t.n, i0 + w.left);
-        const long long seg_first = sh.first + (sh.count - w.left);
-        uint32_t qf[NT][D / 16][2];
+    // q of the next pair is on its way while the last one's states are joined
+    uint32_t qf[NT][D / 16][2];
+    auto load_q = [&](int b, int h) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const bool on = n * 8 + qc < a.G;
@@ -398,6 +398,16 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 qf[n][kk][1] = on ? __ldg(reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8)) : 0u;
             }
         }
+    };
+    load_q(w.b, w.h);
+    int it = 0;
+    bool ok = true;
+    while (ok && w.left > 0) {
+        // ---- one pair's tiles
+        const int b = w.b, h = w.h, i0 = w.i;
+        const Tiles t = w.t;
+        const int i1 = min(t.n, i0 + w.left);
+        const long long seg_first = sh.first + (sh.count - w.left);
         float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -502,8 +512,15 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             w.next(a, TK);
         }
         if (!ok) break;
-        // ---- join the four warps' states and hand the pair's over
-        if (tid == 0) s_dest = segment_dest(a, sh, seg_first, i0, i1, t.n, b, h);
+        if (w.left > 0) load_q(w.b, w.h);
+        // ---- join the four warps' states and hand the pair's over.  The next pair's
+        // join writes slot 2 after a barrier that warp 0 meets once it is done here.
+        Dest ds;
+        if (warp == 0) {
+            if (lane == 0) ds = segment_dest(a, sh, seg_first, i0, i1, t.n, b, h);
+            ds.kind = __shfl_sync(0xffffffffu, ds.kind, 0);
+            ds.slot = __shfl_sync(0xffffffffu, ds.slot, 0);
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -517,7 +534,6 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             bar_consumers<BW * 32>();
             if (warp != 0) continue;
             fold<D>(o[n], m[n], l[n], red + 2 * red_floats<D>(), lane);
-            const Dest ds = s_dest;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int g = n * 8 + qp + j;
@@ -544,7 +560,6 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 }
             }
         }
-        bar_consumers<BW * 32>();                        // s_dest and the buffers are free again
     }
     if (!ok && lane == 0) atomicMin(&r.consumed, it);
     drain(&r);
@@ -607,14 +622,8 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
         return;
     }
     const int grp = lane >> 3, sub = lane & 7, part = warp & 3, g0 = (warp >> 2) * HG;
-    int it = 0;
-    bool ok = true;
-    while (ok && w.left > 0) {
-        const int b = w.b, h = w.h, i0 = w.i;
-        const Tiles t = w.t;
-        const int i1 = min(t.n, i0 + w.left);
-        const long long seg_first = sh.first + (sh.count - w.left);
-        float qr[HG][F::CPL], o[HG][F::CPL], m[HG], l[HG];
+    float qr[HG][F::CPL];
+    auto load_q = [&](int b, int h) {
 #pragma unroll
         for (int g = 0; g < HG; ++g) {
             const bool on = g0 + g < a.G;
@@ -629,6 +638,19 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
                 qr[g][c * 4 + 2] = x.z * f;
                 qr[g][c * 4 + 3] = x.w * f;
             }
+        }
+    };
+    load_q(w.b, w.h);
+    int it = 0;
+    bool ok = true;
+    while (ok && w.left > 0) {
+        const int b = w.b, h = w.h, i0 = w.i;
+        const Tiles t = w.t;
+        const int i1 = min(t.n, i0 + w.left);
+        const long long seg_first = sh.first + (sh.count - w.left);
+        float o[HG][F::CPL], m[HG], l[HG];
+#pragma unroll
+        for (int g = 0; g < HG; ++g) {
             m[g] = -INFINITY;
             l[g] = 0.f;
 #pragma unroll
@@ -706,6 +728,7 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
         }
         if (!ok) break;
         if (tid == 0) s_dest = segment_dest(a, sh, seg_first, i0, i1, t.n, b, h);
+        if (w.left > 0) load_q(w.b, w.h);
         // the warp's four row groups, then the four warps of a head group
 #pragma unroll
         for (int off = 8; off <= 16; off <<= 1)
@@ -827,12 +850,12 @@ int decode_grid(const sa_ctx* ctx, const sa_paged_kv* kv, int hq) {
 }
 
 template <int D>
-static int launch_bf16(cudaStream_t st, int grid, const CUtensorMap& tk, const CUtensorMap& tv, const DecodeArgs& a) {
+static int launch_bf16(cudaStream_t st, int grid, bool overlap, const CUtensorMap& tk, const CUtensorMap& tv, const DecodeArgs& a) {
     auto one = decode_bf16_kernel<D, 1>;
     auto two = decode_bf16_kernel<D, (D < 256 ? 2 : 1)>;
     auto k = a.G <= 8 ? one : two;
     SA_RC_TRY(set_smem_attr_once((const void*)k, bf16_smem<D>()));
-    if (a.to_state) {
+    if (overlap) {
         SA_CUDA_TRY(launch_pdl(k, dim3(grid), dim3(BTHREADS), bf16_smem<D>(), st, tk, tv, a));
     } else {
         k<<<grid, BTHREADS, bf16_smem<D>(), st>>>(tk, tv, a);
@@ -842,7 +865,7 @@ static int launch_bf16(cudaStream_t st, int grid, const CUtensorMap& tk, const C
 }
 
 int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_stride, int hq, int window, int sinks,
-                  float scale, void* out, long long o_stride, bool to_state, const DecodeWs& ws) {
+                  float scale, void* out, long long o_stride, bool to_state, bool overlap, const DecodeWs& ws) {
     DecodeArgs a;
     a.c = make_cache(ctx, kv);
     a.q = q;
@@ -861,7 +884,7 @@ int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q
     if (kv->dtype == SA_F32) {
         const F32Pick p = f32_pick_d(kv->d, a.G);
         SA_RC_TRY(set_smem_attr_once((const void*)p.fn, p.smem));
-        if (to_state) {
+        if (overlap) {
             SA_CUDA_TRY(launch_pdl(p.fn, dim3(grid), dim3(p.threads), p.smem, st, a));
         } else {
             p.fn<<<grid, p.threads, p.smem, st>>>(a);
@@ -873,9 +896,9 @@ int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q
         const int box = std::min(kv->page_size, tile);
         SA_RC_TRY(make_page_tmap(&tk, kv->k_pages, kv, box));
         SA_RC_TRY(make_page_tmap(&tv, kv->v_pages, kv, box));
-        SA_RC_TRY(kv->d == 64    ? launch_bf16<64>(st, grid, tk, tv, a)
-                  : kv->d == 128 ? launch_bf16<128>(st, grid, tk, tv, a)
-                                 : launch_bf16<256>(st, grid, tk, tv, a));
+        SA_RC_TRY(kv->d == 64    ? launch_bf16<64>(st, grid, overlap, tk, tv, a)
+                  : kv->d == 128 ? launch_bf16<128>(st, grid, overlap, tk, tv, a)
+                                 : launch_bf16<256>(st, grid, overlap, tk, tv, a));
     }
     if (to_state) return SA_OK;
     auto join = kv->dtype == SA_F32 ? join_pick<float>(kv->d) : join_pick<__nv_bfloat16>(kv->d);
@@ -943,5 +966,5 @@ SA_API int sa_attn_paged_decode(sa_ctx* ctx, const sa_paged_kv* kv, const void* 
     const size_t need = pg::decode_ws_layout(ctx, kv, hq, false, workspace, &ws);
     SA_CHECK_ARG(workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need,
                  "%s: workspace of %zu bytes (want %zu, 256-byte aligned)", fn, workspace_bytes, need);
-    return pg::decode_launch(ctx, kv, q, q_stride, hq, window, sinks, scale, out, o_stride, false, ws);
+    return pg::decode_launch(ctx, kv, q, q_stride, hq, window, sinks, scale, out, o_stride, false, false, ws);
 }

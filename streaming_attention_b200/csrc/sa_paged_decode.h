@@ -21,9 +21,12 @@ struct DecodeWs {
 int decode_grid(const sa_ctx* ctx, const sa_paged_kv* kv, int hq);
 // Lays the workspace out at `base` (may be null) and returns its size.
 size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool to_state, void* base, DecodeWs* ws);
-// to_state: every pair's state goes to ws (pair, state, slots) and `out` is not written.
+// to_state: every pair's state goes to ws (pair, state, slots) and `out` is not
+// written.  overlap: the stream's last kernel is a shared prefix's, which started
+// after everything that this launch reads was written; the launch may start while
+// it runs.
 int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_stride, int hq, int window, int sinks,
-                  float scale, void* out, long long o_stride, bool to_state, const DecodeWs& ws);
+                  float scale, void* out, long long o_stride, bool to_state, bool overlap, const DecodeWs& ws);
 
 }  // namespace pg
 }  // namespace sa

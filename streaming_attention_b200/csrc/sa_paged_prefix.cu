@@ -183,7 +183,7 @@ SA_API int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const
                                            ws.part_o, ws.part_ml));
         }
     }
-    SA_RC_TRY(pg::decode_launch(ctx, kv, q, q_stride, hq, 0, 0, scale, nullptr, 0, true, ws.own));
+    SA_RC_TRY(pg::decode_launch(ctx, kv, q, q_stride, hq, 0, 0, scale, nullptr, 0, true, prefix_len > 0, ws.own));
     const dim3 grid((unsigned)(kv->n_seqs * (long long)hq));
     auto k = kv->dtype == SA_F32 ? (d == 64 ? pg::prefix_join_kernel<float, 64> : pg::prefix_join_kernel<float, 128>)
                                  : (d == 64 ? pg::prefix_join_kernel<__nv_bfloat16, 64>

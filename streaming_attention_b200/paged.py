@@ -121,7 +121,7 @@ def _workspace(key, like, size_fn, *args):
         if len(_sizes) > 4096:
             _sizes.clear()
         n = _sizes[key] = out.value
-    return like.new_empty(n, dtype=_torch.uint8), n
+    return like.new_empty(-(-n // like.element_size())), n
 
 
 def rope_table(theta: float, rotary_dim: int, n_pos: int, device="cuda", ctx: Context | None = None):
@@ -190,7 +190,7 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, kv_lens, scale: float, w
     qs = _rows(q, "q", n_seqs, None, d, dev, dt)
     hq = q.shape[1]
     if out is None:
-        out, os = q.new_empty((n_seqs, hq, d)), hq * d
+        out, os = _torch.empty_like(q, memory_format=_torch.contiguous_format), hq * d
     else:
         os = _rows(out, "out", n_seqs, hq, d, dev, dt)
     h = _bind(ctx, dev)
@@ -215,7 +215,7 @@ def attn_paged_prefill(q, k_pages, v_pages, block_table, kv_lens, cu_q, scale: f
     hq = q.shape[1]
     cp = _index(cu_q, "cu_q", n_seqs + 1, dev)
     if out is None:
-        out, os = q.new_empty((n, hq, d)), hq * d
+        out, os = _torch.empty_like(q, memory_format=_torch.contiguous_format), hq * d
     else:
         os = _rows(out, "out", n, hq, d, dev, dt)
     check(_lib.sa_attn_paged_prefill(_bind(ctx, dev), kv, q.data_ptr(), qs, n, hq, cp, window, sinks, scale,
@@ -239,7 +239,7 @@ def attn_paged_decode_prefix(q, k_pages, v_pages, prefix_table, prefix_len: int,
     if prefix_table.shape[0] * page < prefix_len:
         raise ValueError(f"prefix_table: {prefix_table.shape[0]} pages of {page} for {prefix_len} rows")
     if out is None:
-        out, os = q.new_empty((n_seqs, hq, d)), hq * d
+        out, os = _torch.empty_like(q, memory_format=_torch.contiguous_format), hq * d
     else:
         os = _rows(out, "out", n_seqs, hq, d, dev, dt)
     h = _bind(ctx, dev)

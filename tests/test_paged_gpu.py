@@ -412,3 +412,227 @@ def test_prefix_reports_bad_pages(dtype):
         assert e.value.code == -6
         sa.attn_paged_decode_prefix(q, pool.kp, pool.vp, pool.table[0], 40, pool.table[1:], pool.kv_lens[1:], 1.0, ctx=ctx)
         ctx.synchronize()
+
+
+def test_a_bad_page_fails_no_later_call():
+    """Bad pages are reported once; other operators on the context go on."""
+    sa = _sa()
+    with sa.Context(0) as ctx:
+        pool = Pool([40], 1, 64, 16, "f32", seed=8, pad_cols=0)
+        q = pool.q(1, 1).cuda()
+        sa.attn_paged_decode(q, pool.kp, pool.vp, pool.table + 1000, pool.kv_lens, 1.0, ctx=ctx)
+        k = torch.randn(1, 50, 64, device="cuda")
+        out = sa.attn_decode(q[0], k, k, 1.0, ctx=ctx)
+        good = sa.attn_paged_decode(q, pool.kp, pool.vp, pool.table, pool.kv_lens, 1.0, ctx=ctx)
+        with pytest.raises(sa.SAError):
+            ctx.synchronize()
+        assert torch.isfinite(out).all() and torch.isfinite(good).all()
+
+
+# ---------------------------------------------------------------- together
+
+def _rope_ref(cos, sin, rot, x, pos, dt):
+    return rotate(x, cos.cpu()[pos], sin.cpu()[pos], rot, False).to(dt)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 4)])
+def test_serving_a_batch(dtype, window, sinks):
+    """Three prompts in ragged chunks, then decode steps, through append and the two attentions: every output
+    against a plain cache of the same tokens."""
+    sa = _sa()
+    hq, hkv, d, page, dt = 4, 2, 64, 16, DT[dtype]
+    prompts, steps = [90, 33, 150], 5
+    max_pages = 12
+    g = torch.Generator().manual_seed(3)
+    kp = torch.full((40, hkv, page, d), math.nan, dtype=dt, device="cuda")
+    vp = kp.clone()
+    table = torch.randperm(40, generator=g)[:36].reshape(3, max_pages).int().cuda()
+    cos, sin = sa.rope_table(1e4, d, 400)
+    plain_k, plain_v = [torch.zeros(hkv, 0, d, dtype=dt) for _ in prompts], [torch.zeros(hkv, 0, d, dtype=dt) for _ in prompts]
+    lens, left = [0, 0, 0], list(prompts)
+    v_max = 5.0
+    while any(left):
+        new = [min(x, n) for x, n in zip(left, (64, 17, 100))]
+        lens = [a + b for a, b in zip(lens, new)]
+        left = [a - b for a, b in zip(left, new)]
+        n = sum(new)
+        qkv = torch.randn(n, hq + 2 * hkv, d, generator=g).to(dt)
+        dev = qkv.cuda()
+        cu = torch.tensor([0] + new).cumsum(0)
+        kv = torch.tensor(lens, dtype=torch.int32).cuda()
+        q = sa.paged_append(dev[:, hq:hq + hkv], dev[:, hq + hkv:], kp, vp, table, kv, cu_q=cu.int().cuda(), q=dev[:, :hq],
+                            rope=(cos, sin))
+        out = sa.attn_paged_prefill(q, kp, vp, table, kv, cu.int().cuda(), d ** -0.5, window=window, sinks=sinks)
+        torch.cuda.synchronize()
+        for b in range(3):
+            r, pos = slice(int(cu[b]), int(cu[b + 1])), torch.arange(lens[b] - new[b], lens[b])
+            plain_k[b] = torch.cat([plain_k[b], _rope_ref(cos, sin, d, qkv[r, hq:hq + hkv], pos, dt).transpose(0, 1)], 1)
+            plain_v[b] = torch.cat([plain_v[b], qkv[r, hq + hkv:].transpose(0, 1)], 1)
+            ref = attend(q[r].cpu(), plain_k[b], plain_v[b], pos, d ** -0.5, window, sinks)
+            _close(out[r], ref, dtype, v_max)
+    for _ in range(steps):
+        lens = [x + 1 for x in lens]
+        kv = torch.tensor(lens, dtype=torch.int32).cuda()
+        qkv = torch.randn(3, hq + 2 * hkv, d, generator=g).to(dt)
+        dev = qkv.cuda()
+        q = sa.paged_append(dev[:, hq:hq + hkv], dev[:, hq + hkv:], kp, vp, table, kv, q=dev[:, :hq], rope=(cos, sin))
+        out = sa.attn_paged_decode(q, kp, vp, table, kv, d ** -0.5, window=window, sinks=sinks)
+        torch.cuda.synchronize()
+        for b in range(3):
+            pos = torch.tensor([lens[b] - 1])
+            plain_k[b] = torch.cat([plain_k[b], _rope_ref(cos, sin, d, qkv[b:b + 1, hq:hq + hkv], pos, dt).transpose(0, 1)], 1)
+            plain_v[b] = torch.cat([plain_v[b], qkv[b:b + 1, hq + hkv:].transpose(0, 1)], 1)
+            _close(out[b:b + 1], attend(q[b:b + 1].cpu(), plain_k[b], plain_v[b], [lens[b] - 1], d ** -0.5, window, sinks),
+                   dtype, v_max)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_beams_behind_a_prompt(dtype):
+    """Four continuations of one prompt: the prompt prefilled once, their own tokens appended behind it."""
+    sa = _sa()
+    hq, hkv, d, page, dt, n = 8, 2, 128, 32, DT[dtype], 4
+    P = 205
+    pool = Pool([P], hkv, d, page, dtype, seed=21, extra_pages=12)
+    cos, sin = sa.rope_table(1e4, d, 400)
+    own = torch.tensor(pool.free[:8], dtype=torch.int32).reshape(n, 2).cuda()
+    plain_k, plain_v = torch.zeros(n, hkv, 0, d, dtype=dt), torch.zeros(n, hkv, 0, d, dtype=dt)
+    for step in range(1, 36):
+        qkv = torch.randn(n, hq + 2 * hkv, d, generator=pool.gen).to(dt)
+        dev = qkv.cuda()
+        kv = torch.full((n,), step, dtype=torch.int32, device="cuda")
+        q = sa.paged_append(dev[:, hq:hq + hkv], dev[:, hq + hkv:], pool.kp, pool.vp, own, kv, q=dev[:, :hq], rope=(cos, sin),
+                            pos0=P)
+        plain_k = torch.cat([plain_k, _rope_ref(cos, sin, d, qkv[:, hq:hq + hkv], torch.full((n,), P + step - 1), dt)[:, :, None]], 2)
+        plain_v = torch.cat([plain_v, qkv[:, hq + hkv:][:, :, None]], 2)
+        if step in (1, 2, 32, 33, 35):
+            out = sa.attn_paged_decode_prefix(q, pool.kp, pool.vp, pool.table[0], P, own, kv, d ** -0.5)
+            torch.cuda.synchronize()
+            for b in range(n):
+                ref = attend(q[b:b + 1].cpu(), torch.cat([pool.k[0], plain_k[b]], 1), torch.cat([pool.v[0], plain_v[b]], 1),
+                             [P + step - 1], d ** -0.5)
+                _close(out[b:b + 1], ref, dtype, max(_v_max(pool), 6.0), (step, b))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_captured_calls_follow_lengths_and_tables(dtype):
+    """A captured step replayed after the lengths, the tables and the rows changed; two graphs with their own
+    workspaces replayed on two streams at once."""
+    sa = _sa()
+    pool = Pool([500, 40, 900], 2, 64, 16, dtype, seed=30, extra_pages=70, pad_cols=10)
+    q = pool.q(3, 4)
+    qd = q.cuda()
+    kv, table = pool.kv_lens.clone(), pool.table.clone()
+    tok = pool.q(7, 4)
+    tokd, cu = tok.cuda(), torch.tensor([0, 3, 4, 7], dtype=torch.int32).cuda()
+
+    def step():
+        return (sa.attn_paged_decode(qd, pool.kp, pool.vp, table, kv, 0.125, window=300, sinks=2),
+                sa.attn_paged_prefill(tokd, pool.kp, pool.vp, table, kv, cu, 0.125),
+                sa.attn_paged_decode_prefix(qd, pool.kp, pool.vp, pool.table[0], 500, table, kv, 0.125))
+
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    with torch.cuda.stream(side):
+        step()
+        torch.cuda.synchronize()
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(step())
+            graphs.append(g)
+    other = torch.cuda.Stream()
+    for lens in ([500, 40, 900], [17, 0, 640], [499, 39, 1]):
+        kv.copy_(torch.tensor(lens, dtype=torch.int32))
+        table.copy_(pool.table)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            with torch.cuda.stream(side):
+                graphs[0].replay()
+            with torch.cuda.stream(other):
+                graphs[1].replay()
+        torch.cuda.synchronize()
+        dec = torch.cat([attend(q[b:b + 1], pool.k[b][:, :n], pool.v[b][:, :n], [n - 1], 0.125, 300, 2) for b, n in enumerate(lens)])
+        new = [3, 1, 3]
+        at = [0, 3, 4, 7]
+        pre = torch.cat([attend(tok[at[b]:at[b + 1]], pool.k[b][:, :n], pool.v[b][:, :n], list(range(n - new[b], n)), 0.125)
+                         for b, n in enumerate(lens)])
+        fix = torch.cat([attend(q[b:b + 1], torch.cat([pool.k[0], pool.k[b][:, :n]], 1), torch.cat([pool.v[0], pool.v[b][:, :n]], 1),
+                                [500 + n - 1], 0.125) for b, n in enumerate(lens)])
+        for o in outs:
+            for got, ref in zip(o, (dec, pre, fix)):
+                _close(got, ref, dtype, _v_max(pool), lens)
+    del graphs
+
+
+def test_out_may_be_the_queries():
+    sa = _sa()
+    for dtype in ("bf16", "f32"):
+        pool = Pool([700, 33], 2, 128, 16, dtype, seed=31)
+        q, t = pool.q(2, 8).cuda(), pool.q(300, 8).cuda()
+        cu = torch.tensor([0, 280, 300], dtype=torch.int32).cuda()
+        args = (pool.kp, pool.vp, pool.table, pool.kv_lens)
+        for f in (lambda x, o: sa.attn_paged_decode(x, *args, 0.1, out=o),
+                  lambda x, o: sa.attn_paged_decode_prefix(x, pool.kp, pool.vp, pool.table[0], 650, pool.table, pool.kv_lens, 0.1, out=o)):
+            want, got = f(q, None), q.clone()
+            assert f(got, got) is got
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+        want, got = sa.attn_paged_prefill(t, *args, cu, 0.1), t.clone()
+        sa.attn_paged_prefill(got, *args, cu, 0.1, out=got)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_pools_past_32_bit_offsets():
+    """Pages 2^31 elements apart: offsets of 2^32 elements and 2^33 bytes in every operator."""
+    sa = _sa()
+    page, d, hkv, far = 16, 64, 2, 1 << 31
+    lens = [40, 20]
+    for dtype in ("bf16", "f32"):
+        small = Pool(lens, hkv, d, page, dtype, seed=33, extra_pages=0)
+        n_pages = 3
+        raw = torch.empty((n_pages - 1) * far + 2 * hkv * page * d, dtype=DT[dtype], device="cuda")
+        k = raw.as_strided((n_pages, hkv, page, d), (far, page * d, d, 1))
+        v = raw.as_strided((n_pages, hkv, page, d), (far, page * d, d, 1), hkv * page * d)
+        # sequence 0 in pages 2, 0, 1
+        table = torch.tensor([[2, 0, 1]], dtype=torch.int32).cuda()
+        kv = torch.tensor([40], dtype=torch.int32).cuda()
+        rows = torch.cat([small.k[0], small.v[0]]).transpose(0, 1).contiguous().cuda()      # [40, 2 hkv, d]
+        cu = torch.tensor([0, 40], dtype=torch.int32).cuda()
+        sa.paged_append(rows[:, :hkv], rows[:, hkv:], k, v, table, kv, cu_q=cu)
+        assert torch.equal(k[2, :, :].cpu(), small.k[0][:, :16]) and torch.equal(v[1, :, :8].cpu(), small.v[0][:, 32:])
+        q = small.q(40, 4)
+        out = sa.attn_paged_prefill(q.cuda(), k, v, table, kv, cu, 0.125)
+        _close(out, attend(q, small.k[0], small.v[0], range(40), 0.125), dtype, _v_max(small))
+        out = sa.attn_paged_decode(q[:1].cuda(), k, v, table, kv, 0.125)
+        _close(out, attend(q[:1], small.k[0], small.v[0], [39], 0.125), dtype, _v_max(small))
+        out = sa.attn_paged_decode_prefix(q[:1].cuda(), k, v, table[0], 39, table, kv, 0.125)
+        both = [torch.cat([x[:, :39], x], 1) for x in (small.k[0], small.v[0])]
+        _close(out, attend(q[:1], *both, [78], 0.125), dtype, _v_max(small))
+        del raw, k, v
+
+
+def test_python_wrappers_check_gpu_tensors():
+    sa = _sa()
+    pool = Pool([5, 5], 2, 64, 16, "bf16", seed=1)
+    args = (pool.kp, pool.vp, pool.table, pool.kv_lens)
+    q = pool.q(2, 4).cuda()
+    for bad, exc in ((q.float(), TypeError), (q[:1], ValueError), (q[:, :, :32], ValueError),
+                     (q.transpose(1, 2).contiguous().transpose(1, 2), ValueError), (q.cpu(), ValueError), (q[:, :3], sa.SAError)):
+        with pytest.raises(exc):
+            sa.attn_paged_decode(bad, *args, 0.1)
+    for over in (dict(block_table=pool.table.long()), dict(block_table=pool.table[:1]), dict(kv_lens=pool.kv_lens.float()),
+                 dict(kv_lens=pool.kv_lens[:1]), dict(v_pages=pool.vp.float()), dict(k_pages=pool.kp.transpose(1, 2))):
+        kw = dict(zip(("k_pages", "v_pages", "block_table", "kv_lens"), args)) | over
+        with pytest.raises((ValueError, TypeError)):
+            sa.attn_paged_decode(q, scale=0.1, **kw)
+    with pytest.raises(ValueError):
+        sa.attn_paged_prefill(q, *args, torch.tensor([0, 1], dtype=torch.int32).cuda(), 0.1)
+    with pytest.raises(ValueError):
+        sa.attn_paged_decode_prefix(q, pool.kp, pool.vp, pool.table[0], 10000, pool.table, pool.kv_lens, 0.1)
+    with pytest.raises(ValueError):
+        sa.paged_append(q[:1, :2], q[:1, 2:], *args)                       # two sequences, one token, no cu_q
+    with pytest.raises(ValueError):
+        sa.attn_paged_decode(q, *args, 0.1, out=q[:, :2])
+    torch.cuda.synchronize()
