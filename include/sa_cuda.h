@@ -376,12 +376,15 @@ int sa_attn_decode_noalloc(void* stream, int dtype, const void* q, const void* k
  * accessed (its rows' contribution is undefined), and sa_ctx_synchronize then
  * returns SA_ERR_RANGE.
  *
- * Workspaces are the caller's (256-byte aligned device memory, contents
- * arbitrary); calls that may run at the same time, captured ones included,
- * need workspaces of their own.  Their sizes depend on the shapes in kv and on
- * hq (and n_tokens), not on lengths.
+ * Workspaces are the caller's (256-byte aligned device memory); calls that may
+ * run at the same time, captured ones included, need workspaces of their own.
+ * Their sizes depend on the shapes in kv and on hq, not on lengths.  The first
+ * SA_PAGED_ZERO_BYTES of that of sa_attn_paged_decode are zeros before its first
+ * use; every call, of any shape, leaves them zero for the next.  All else may
+ * hold anything.  out may be q.
  */
 #define SA_PAGED_MAX_SEQS 65536
+#define SA_PAGED_ZERO_BYTES 4096
 typedef struct {
     void* k_pages;
     void* v_pages;

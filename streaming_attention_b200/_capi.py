@@ -26,6 +26,7 @@ SA_HOST_PTRS = 1
 SA_KV_STATIC = 2
 
 SA_PAGED_MAX_SEQS = 65536
+SA_PAGED_ZERO_BYTES = 4096
 
 _vp = C.c_void_p
 _fp = C.POINTER(C.c_float)

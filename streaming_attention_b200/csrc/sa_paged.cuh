@@ -57,7 +57,7 @@ struct Joined {
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = 0.f;
     }
-    // ml(p) -> (m, l) of part p;  row(p) -> its O row
+    // ml(p) -> (m, l) of part p, read past the L1 cache;  row(p) -> its O row
     template <typename ML, typename ROW>
     __device__ __forceinline__ void add(int parts, int lane, ML ml, ROW row) {
         for (int base = 0; base < parts; base += 32) {
@@ -79,16 +79,16 @@ struct Joined {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     wi[i] = __shfl_sync(0xffffffffu, w, (i0 + i) & 31);
-                    const bool on = i0 + i < n && wi[i] > 0.f;      // the O of an empty part is not written
+                    const bool on = i0 + i < n && wi[i] != 0.f;     // the O of an empty part is not written
                     const float* r = on ? row(base + i0 + i) + lane * V : nullptr;
                     if (!on) wi[i] = 0.f;
                     if constexpr (V == 2) {
-                        const float2 y = on ? *reinterpret_cast<const float2*>(r) : make_float2(0.f, 0.f);
+                        const float2 y = on ? __ldcg(reinterpret_cast<const float2*>(r)) : make_float2(0.f, 0.f);
                         v[i][0] = y.x; v[i][1] = y.y;
                     } else {
 #pragma unroll
                         for (int c = 0; c < V; c += 4) {
-                            const float4 y = on ? *reinterpret_cast<const float4*>(r + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            const float4 y = on ? __ldcg(reinterpret_cast<const float4*>(r + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
                             v[i][c] = y.x; v[i][c + 1] = y.y; v[i][c + 2] = y.z; v[i][c + 3] = y.w;
                         }
                     }
@@ -116,12 +116,10 @@ struct Joined {
         for (int off = 16; off; off >>= 1) t += __shfl_xor_sync(0xffffffffu, t, off);
         return t;
     }
-    // The lane's columns of the normalised row (NaN after an expired wait), in OT.
+    // The lane's columns of the normalised row, in OT.
     template <typename OT>
-    __device__ __forceinline__ void store(OT* dst, int lane, const int* status) const {
-        const float t = total();
-        const bool failed = *reinterpret_cast<const volatile int*>(status) == SA_STATUS_TIMEOUT;
-        const float f = failed ? nanf("") : (t > 0.f ? 1.f / t : 0.f);
+    __device__ __forceinline__ void store(OT* dst, int lane) const {
+        const float t = total(), f = t == 0.f ? 0.f : 1.f / t;
         dst += lane * V;
         if constexpr (sizeof(OT) == 4) {
 #pragma unroll

@@ -14,7 +14,8 @@
 // the device, so the host neither knows the lengths nor plans again when they
 // grow (a captured launch stays right).  Only the first and the last (sequence,
 // head) of a CTA can be shared with other CTAs; such shares leave their
-// (m, l, O) in the workspace, and the second kernel joins them.
+// (m, l, O) in the workspace, and the CTA that hands in a pair's last one joins
+// them (in the order of the rows, so the result does not depend on who is last).
 //
 // A producer warp copies tiles of 32 KB (64 KB at d = 256) into a ring of three;
 // its lanes fetch the block-table entries of the next tile while the ring is
@@ -167,30 +168,26 @@ struct Dest {
     int kind, slot;
 };
 
-// Called by one thread when a CTA has finished tiles [.., i_end] of a pair:
-// decides where its state goes and leaves the record that the join needs.
-__device__ __forceinline__ Dest segment_dest(const DecodeArgs& a, const Share& s, long long seg_first, int i0, int i1,
-                                             int n, int b, int h) {
+__device__ __forceinline__ Dest segment_dest(const DecodeArgs& a, const Share& s, long long seg_first, bool whole,
+                                             int b, int h) {
     Dest d;
-    const bool whole = i0 == 0 && i1 == n;
-    const long long t0 = seg_first - i0, t1 = t0 + n;               // the pair's tiles in the list
-    const int pair = b * a.c.hkv + h;
-    if (whole) {
-        d.kind = a.to_state ? TO_STATE : TO_OUT;
-        d.slot = pair;
-        if (a.to_state) a.ws.pair[pair] = make_int4(-1, 0, 0, 0);
-        return d;
-    }
-    const int which = seg_first == s.first ? 0 : 1;
-    d.kind = TO_SLOT;
-    d.slot = 2 * blockIdx.x + which;
-    if (i0 == 0) {                                                   // this CTA holds the pair's first tile
-        const int4 rec = make_int4(blockIdx.x, share_of(t1 - 1, s.total, s.n_ctas), which, pair);
-        if (a.to_state) a.ws.pair[pair] = rec;
-        else a.ws.head[blockIdx.x] = rec;
-    }
+    d.kind = !whole ? TO_SLOT : a.to_state ? TO_STATE : TO_OUT;
+    d.slot = whole ? b * a.c.hkv + h : 2 * (int)blockIdx.x + (seg_first == s.first ? 0 : 1);
     return d;
 }
+// The shares of a pair whose tiles begin at t0 in the list: CTAs first .. last,
+// the first one's in slot `slot`, the others' in slot 0.
+struct Shares {
+    int first, last, slot;
+};
+__device__ __forceinline__ Shares pair_shares(const Share& s, long long t0, int n) {
+    Shares x;
+    x.first = share_of(t0, s.total, s.n_ctas);
+    x.last = share_of(t0 + n - 1, s.total, s.n_ctas);
+    x.slot = share_first(x.first, s.total, s.n_ctas) == t0 ? 0 : 1;
+    return x;
+}
+__device__ __forceinline__ long long share_slot(const Shares& x, int p) { return 2LL * (x.first + p) + (p == 0 ? x.slot : 0); }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -223,7 +220,53 @@ struct Ring {
     long long scan[40];
     Share share;
     int issued, consumed;
+    int failed;              // a consumer's wait expired: what follows is NaN
+    int last;                // this CTA handed in a pair's last share
 };
+
+// A consumer warp's wait for tile `it` of its share; the first that expires is
+// noted, and no further one is waited for.
+__device__ __forceinline__ bool consume_wait(Ring* r, int it, bool& ok, int* status) {
+    if (!ok) return false;
+    if ((ok = mbar_wait(r->full + it % STAGES, (it / STAGES) & 1, status))) return true;
+    atomicMin(&r->consumed, it);
+    r->failed = 1;
+    return false;
+}
+
+// With a prefix to come: where the join finds a pair's state.
+__device__ __forceinline__ void record_pair(const DecodeArgs& a, const Share& s, long long t0, int n, int i0, bool whole,
+                                            int b, int h) {
+    const int pair = b * a.c.hkv + h;
+    if (whole) {
+        a.ws.pair[pair] = make_int4(-1, 0, 0, 0);
+    } else if (i0 == 0) {
+        const Shares x = pair_shares(s, t0, n);
+        a.ws.pair[pair] = make_int4(x.first, x.last, x.slot, 0);
+    }
+}
+
+// The consumer threads have written a share's state (thread 0's warp did): count
+// it, and where it was the pair's last, join the pair: a warp per query head.
+template <typename OT, int D, int NT>
+__device__ __forceinline__ void hand_in(const DecodeArgs& a, Ring* r, const Share& sh, long long t0, int n, int b, int h) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Shares x = pair_shares(sh, t0, n);
+    const int parts = x.last - x.first + 1;
+    __threadfence();
+    bar_consumers<NT>();
+    if (threadIdx.x == 0) r->last = atomicAdd(a.ws.count + x.first, 1u) == (unsigned)(parts - 1);
+    bar_consumers<NT>();
+    if (!r->last) return;
+    __threadfence();
+    if (threadIdx.x == 0) a.ws.count[x.first] = 0u;
+    for (int g = warp; g < a.G; g += NT / 32) {
+        Joined<D> s;
+        s.add(parts, lane, [&](int p) { return __ldcg(a.ws.slot_ml + share_slot(x, p) * a.G + g); },
+              [&](int p) { return a.ws.slot_o + (share_slot(x, p) * a.G + g) * D; });
+        s.store(static_cast<OT*>(a.out) + (long long)b * a.o_stride + (long long)(h * a.G + g) * D, lane);
+    }
+}
 
 // The producer warp: copies this share's tiles, pages that hold no visible row
 // left out.  bf16 tiles through the tensor maps (swizzled for ldmatrix), fp32
@@ -362,7 +405,7 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
         fence_barrier_init();
         r.issued = 0;
-        if (!a.to_state) a.ws.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        r.failed = 0;
     }
     plan_share<BTHREADS>(a, TK, &r.share, r.scan);
     const Share sh = r.share;
@@ -400,9 +443,11 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
     };
     load_q(w.b, w.h);
+    // After an expired wait the walk goes on without its tiles, so that the warps
+    // meet at every barrier and every share is handed in (as NaN).
     int it = 0;
     bool ok = true;
-    while (ok && w.left > 0) {
+    while (w.left > 0) {
         // ---- one pair's tiles
         const int b = w.b, h = w.h, i0 = w.i;
         const Tiles t = w.t;
@@ -420,7 +465,10 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
         for (int i = i0; i < i1; ++i, ++it) {
             const int s = it % STAGES;
-            if (!(ok = mbar_wait(r.full + s, (it / STAGES) & 1, a.c.status))) break;
+            if (!consume_wait(&r, it, ok, a.c.status)) {
+                w.next(a, TK);
+                continue;
+            }
             const uint32_t ks = sbuf + s * Z::STAGE_BYTES, vs = ks + Z::STAGE_BYTES / 2;
             const int row0 = t.row0(i, TK);
 #pragma unroll
@@ -511,16 +559,11 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             if (lane == 0) mbar_arrive(r.empty + s);
             w.next(a, TK);
         }
-        if (!ok) break;
         if (w.left > 0) load_q(w.b, w.h);
         // ---- join the four warps' states and hand the pair's over.  The next pair's
         // join writes slot 2 after a barrier that warp 0 meets once it is done here.
-        Dest ds;
-        if (warp == 0) {
-            if (lane == 0) ds = segment_dest(a, sh, seg_first, i0, i1, t.n, b, h);
-            ds.kind = __shfl_sync(0xffffffffu, ds.kind, 0);
-            ds.slot = __shfl_sync(0xffffffffu, ds.slot, 0);
-        }
+        const bool whole = i0 == 0 && i1 == t.n;
+        const Dest ds = segment_dest(a, sh, seg_first, whole, b, h);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -534,12 +577,17 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             bar_consumers<BW * 32>();
             if (warp != 0) continue;
             fold<D>(o[n], m[n], l[n], red + 2 * red_floats<D>(), lane);
+            const bool failed = *reinterpret_cast<volatile int*>(&r.failed) != 0;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int g = n * 8 + qp + j;
                 if (g >= a.G) continue;
+                if (failed) {
+                    m[n][j] = 0.f;
+                    l[n][j] = nanf("");
+                }
                 if (ds.kind == TO_OUT) {
-                    const float inv = l[n][j] > 0.f ? 1.f / l[n][j] : 0.f;
+                    const float inv = 1.f / l[n][j];     // the pair's query sees its own row at least
                     __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + (long long)b * a.o_stride +
                                          (long long)(h * a.G + g) * D + qc;
 #pragma unroll
@@ -560,8 +608,12 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 }
             }
         }
+        if (a.to_state) {
+            if (tid == 0) record_pair(a, sh, seg_first - i0, t.n, i0, whole, b, h);
+        } else if (!whole) {
+            hand_in<__nv_bfloat16, D, BW * 32>(a, &r, sh, seg_first - i0, t.n, b, h);
+        }
     }
-    if (!ok && lane == 0) atomicMin(&r.consumed, it);
     drain(&r);
     leave(a);
 }
@@ -589,7 +641,6 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
     constexpr int TK = Z::TK, NW = NG * 4, THREADS = (NW + 1) * 32;
     extern __shared__ unsigned char smem_raw[];
     __shared__ Ring r;
-    __shared__ Dest s_dest;
     unsigned char* buf = smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u);
     float* red = reinterpret_cast<float*>(buf + STAGES * Z::STAGE_BYTES);   // [warp][HG][D + 2]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -601,7 +652,7 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
         }
         fence_barrier_init();
         r.issued = 0;
-        if (!a.to_state) a.ws.head[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        r.failed = 0;
     }
     plan_share<THREADS>(a, TK, &r.share, r.scan);
     const Share sh = r.share;
@@ -643,7 +694,7 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
     load_q(w.b, w.h);
     int it = 0;
     bool ok = true;
-    while (ok && w.left > 0) {
+    while (w.left > 0) {
         const int b = w.b, h = w.h, i0 = w.i;
         const Tiles t = w.t;
         const int i1 = min(t.n, i0 + w.left);
@@ -658,7 +709,10 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
         }
         for (int i = i0; i < i1; ++i, ++it) {
             const int s = it % STAGES;
-            if (!(ok = mbar_wait(r.full + s, (it / STAGES) & 1, a.c.status))) break;
+            if (!consume_wait(&r, it, ok, a.c.status)) {
+                w.next(a, TK);
+                continue;
+            }
             const unsigned char* ks = buf + s * Z::STAGE_BYTES;
             const unsigned char* vs = ks + Z::STAGE_BYTES / 2;
             const int row0 = t.row0(i, TK);
@@ -726,8 +780,8 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
             if (lane == 0) mbar_arrive(r.empty + s);
             w.next(a, TK);
         }
-        if (!ok) break;
-        if (tid == 0) s_dest = segment_dest(a, sh, seg_first, i0, i1, t.n, b, h);
+        const bool whole = i0 == 0 && i1 == t.n;
+        const Dest ds = segment_dest(a, sh, seg_first, whole, b, h);
         if (w.left > 0) load_q(w.b, w.h);
         // the warp's four row groups, then the four warps of a head group
 #pragma unroll
@@ -760,7 +814,7 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
             }
         }
         bar_consumers<NW * 32>();
-        const Dest ds = s_dest;
+        const bool failed = *reinterpret_cast<volatile int*>(&r.failed) != 0;
         for (int idx = tid; idx < a.G * D; idx += NW * 32) {
             const int g = idx / D, col = idx - g * D;
             const float* src = red + ((g / HG) * 4 * HG + g % HG) * (D + 2);       // + HG rows per warp
@@ -775,44 +829,27 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
                 L += y[D + 1] * wt;
                 O += y[col] * wt;
             }
+            if (failed) {
+                M = 0.f;
+                L = nanf("");
+            }
             if (ds.kind == TO_OUT) {
-                static_cast<float*>(a.out)[(long long)b * a.o_stride + (long long)(h * a.G + g) * D + col] =
-                    L > 0.f ? O / L : 0.f;
+                static_cast<float*>(a.out)[(long long)b * a.o_stride + (long long)(h * a.G + g) * D + col] = O / L;
             } else {
                 const long long at = (long long)ds.slot * a.G + g;
                 (ds.kind == TO_STATE ? a.ws.state_o : a.ws.slot_o)[at * D + col] = O;
                 if (col == 0) (ds.kind == TO_STATE ? a.ws.state_ml : a.ws.slot_ml)[at] = make_float2(M, L);
             }
         }
-        bar_consumers<NW * 32>();
+        if (a.to_state) {
+            if (tid == 0) record_pair(a, sh, seg_first - i0, t.n, i0, whole, b, h);
+        } else if (!whole) {
+            hand_in<float, D, NW * 32>(a, &r, sh, seg_first - i0, t.n, b, h);
+        }
+        bar_consumers<NW * 32>();                        // the buffers are free again
     }
-    if (!ok && lane == 0) atomicMin(&r.consumed, it);
     drain(&r);
     leave(a);
-}
-
-// ---- the join ----------------------------------------------------------------
-// CTA c joins the shares of the pair whose first tile CTA c of the decode held
-// and whose last one it did not, if there is such a pair; a warp per query head.
-constexpr int JW = 4;
-template <typename OT, int D>
-__global__ void __launch_bounds__(JW * 32) join_kernel(const __grid_constant__ DecodeArgs a) {
-    pdl_wait();
-    const int4 rec = a.ws.head[blockIdx.x];
-    if (rec.x < 0) return;
-    const int lane = threadIdx.x & 31;
-    const int b = rec.w / a.c.hkv, h = rec.w - b * a.c.hkv;
-    for (int g = threadIdx.x >> 5; g < a.G; g += JW) {
-        auto at = [&](int p) { return (2LL * (rec.x + p) + (p == 0 ? rec.z : 0)) * a.G + g; };
-        Joined<D> s;
-        s.add(rec.y - rec.x + 1, lane, [&](int p) { return a.ws.slot_ml[at(p)]; },
-              [&](int p) { return a.ws.slot_o + at(p) * D; });
-        s.store(static_cast<OT*>(a.out) + (long long)b * a.o_stride + (long long)(h * a.G + g) * D, lane, a.c.status);
-    }
-}
-template <typename OT>
-static auto join_pick(int d) {
-    return d == 64 ? join_kernel<OT, 64> : d == 128 ? join_kernel<OT, 128> : join_kernel<OT, 256>;
 }
 
 using F32Fn = void (*)(const DecodeArgs);
@@ -845,8 +882,8 @@ static F32Pick f32_pick_d(int d, int G) {
 
 // CTAs of a decode launch: as many as fit the GPU at once.
 int decode_grid(const sa_ctx* ctx, const sa_paged_kv* kv, int hq) {
-    if (kv->dtype == SA_F32) return ctx->num_sms * f32_pick_d(kv->d, hq / kv->hkv).ctas;
-    return ctx->num_sms * (kv->d == 256 ? 1 : 2);
+    const int ctas = kv->dtype == SA_F32 ? f32_pick_d(kv->d, hq / kv->hkv).ctas : (kv->d == 256 ? 1 : 2);
+    return std::min(ctx->num_sms * ctas, SA_PAGED_ZERO_BYTES / 4);
 }
 
 template <int D>
@@ -900,14 +937,11 @@ int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q
                   : kv->d == 128 ? launch_bf16<128>(st, grid, overlap, tk, tv, a)
                                  : launch_bf16<256>(st, grid, overlap, tk, tv, a));
     }
-    if (to_state) return SA_OK;
-    auto join = kv->dtype == SA_F32 ? join_pick<float>(kv->d) : join_pick<__nv_bfloat16>(kv->d);
-    SA_CUDA_TRY(launch_pdl(join, dim3(grid), dim3(JW * 32), 0, st, a));
     return SA_OK;
 }
 
 size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool to_state, void* base, DecodeWs* ws) {
-    const int grid = decode_grid(ctx, kv, hq), G = hq / kv->hkv;
+    const int grid = decode_grid(ctx, kv, hq), G = hq / kv->hkv;      // grid <= SA_PAGED_ZERO_BYTES / 4
     const size_t slots = (size_t)grid * 2 * G, rows = (size_t)kv->n_seqs * hq, d4 = (size_t)kv->d * 4;
     size_t at = 0;
     unsigned char* p = static_cast<unsigned char*>(base);
@@ -917,14 +951,14 @@ size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool t
         return p ? p + o : nullptr;
     };
     DecodeWs w = {};
+    // first, and as long for every shape: calls of other shapes leave it zero too
+    if (!to_state) w.count = reinterpret_cast<unsigned*>(take(SA_PAGED_ZERO_BYTES));
     w.slot_o = reinterpret_cast<float*>(take(slots * d4));
     w.slot_ml = reinterpret_cast<float2*>(take(slots * 8));
     if (to_state) {
         w.pair = reinterpret_cast<int4*>(take((size_t)kv->n_seqs * kv->hkv * sizeof(int4)));
         w.state_o = reinterpret_cast<float*>(take(rows * d4));
         w.state_ml = reinterpret_cast<float2*>(take(rows * 8));
-    } else {
-        w.head = reinterpret_cast<int4*>(take((size_t)grid * sizeof(int4)));
     }
     w.d = kv->d;
     w.out_elt = kv->dtype == SA_F32 ? 4 : 2;

@@ -11,8 +11,8 @@ namespace pg {
 struct DecodeWs {
     float* slot_o;    // [grid][2][G][d]: the first and the last pair of a CTA
     float2* slot_ml;  // [grid][2][G]
-    int4* head;       // [grid]: first CTA, last CTA, first CTA's slot, pair; first CTA -1: nothing to join
-    int4* pair;       // [n_seqs * hkv] the same by pair (first CTA -1: the state is whole), with `state`
+    unsigned* count;  // [grid]: shares handed in of the pair whose first one the CTA holds; zero between calls
+    int4* pair;       // [n_seqs * hkv]: first CTA (-1: the state is whole), last CTA, first CTA's slot; with `state`
     float* state_o;   // [n_seqs][hq][d]
     float2* state_ml; // [n_seqs][hq]
     int d, out_elt;

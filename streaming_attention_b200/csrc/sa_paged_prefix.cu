@@ -43,15 +43,15 @@ __global__ void __launch_bounds__(JT) prefix_join_kernel(const __grid_constant__
     const int b = (int)(row / a.hq), h = (int)(row - (long long)b * a.hq), kvh = h / a.G, g = h - kvh * a.G;
     const int p0 = warp * a.parts / W, p1 = (warp + 1) * a.parts / W;
     Joined<D> s;
-    s.add(p1 - p0, lane, [&](int p) { return reinterpret_cast<const float2*>(a.part_ml)[(p0 + p) * rows + row]; },
+    s.add(p1 - p0, lane, [&](int p) { return __ldcg(reinterpret_cast<const float2*>(a.part_ml) + (p0 + p) * rows + row); },
           [&](int p) { return a.part_o + ((p0 + p) * rows + row) * D; });
     if (warp == W - 1 && seq_len(a.c, b) > 0) {
         const int4 rec = a.ws.pair[b * a.c.hkv + kvh];
         if (rec.x < 0) {
-            s.add(1, lane, [&](int) { return a.ws.state_ml[row]; }, [&](int) { return a.ws.state_o + row * D; });
+            s.add(1, lane, [&](int) { return __ldcg(a.ws.state_ml + row); }, [&](int) { return a.ws.state_o + row * D; });
         } else {
             auto at = [&](int p) { return (2LL * (rec.x + p) + (p == 0 ? rec.z : 0)) * a.G + g; };
-            s.add(rec.y - rec.x + 1, lane, [&](int p) { return a.ws.slot_ml[at(p)]; },
+            s.add(rec.y - rec.x + 1, lane, [&](int p) { return __ldcg(a.ws.slot_ml + at(p)); },
                   [&](int p) { return a.ws.slot_o + at(p) * D; });
         }
     }
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(JT) prefix_join_kernel(const __grid_constant__
     if (warp > 0) return;
 #pragma unroll
     for (int w = 0; w < W - 1; ++w) s.add_one(lane, s_ml[w].x, s_ml[w].y, s_o[w]);
-    s.store(static_cast<OT*>(a.out) + (long long)b * a.o_stride + (long long)h * D, lane, a.c.status);
+    s.store(static_cast<OT*>(a.out) + (long long)b * a.o_stride + (long long)h * D, lane);
 }
 
 struct PrefixWs {

@@ -13,8 +13,8 @@ the pages' device, asynchronously.
   cu_q              [n_seqs + 1] int32: sequence b's tokens are rows
                     cu_q[b] .. cu_q[b + 1] - 1 of the token tensors
 
-Each call takes its workspace from torch's allocator, so calls on different
-streams and calls captured into different graphs do not share one.
+Workspaces come from torch's allocator: calls on different streams and calls
+captured into different graphs do not share one.
 
 A decode step of a small batch takes the GPU some ten microseconds, so the
 wrappers are written to cost the host less than that: one look at each
@@ -26,11 +26,12 @@ from __future__ import annotations
 import ctypes as C
 import struct
 
-from ._capi import SA_BF16, SA_F32, Context, check, default_context, lib
+from ._capi import SA_BF16, SA_F32, SA_PAGED_ZERO_BYTES, Context, check, default_context, lib
 
 _torch = None
 _lib = None
 _sizes: dict = {}
+_decode_ws: dict = {}
 # the members of sa_paged_kv in order, natively aligned
 _pack = struct.Struct("@PPiiiiiqPqiPi").pack
 
@@ -113,7 +114,7 @@ def _bind(ctx: Context | None, dev: int):
     return ctx.h
 
 
-def _workspace(key, like, size_fn, *args):
+def _size(key, size_fn, *args) -> int:
     n = _sizes.get(key)
     if n is None:
         out = C.c_size_t()
@@ -121,7 +122,20 @@ def _workspace(key, like, size_fn, *args):
         if len(_sizes) > 4096:
             _sizes.clear()
         n = _sizes[key] = out.value
-    return like.new_empty(-(-n // like.element_size())), n
+    return n
+
+
+def _decode_workspace(dev: int, n: int):
+    """The decode's workspace, its head zero: kept from call to call of a stream; a captured call has its own."""
+    if _torch._C._cuda_isCurrentStreamCapturing():
+        ws = _torch.empty(n, dtype=_torch.uint8, device=dev)
+        ws[:SA_PAGED_ZERO_BYTES].zero_()
+        return ws
+    key = (dev, _torch._C._cuda_getCurrentRawStream(dev))
+    ws = _decode_ws.get(key)
+    if ws is None or ws.numel() < n:
+        ws = _decode_ws[key] = _torch.zeros(n, dtype=_torch.uint8, device=dev)
+    return ws
 
 
 def rope_table(theta: float, rotary_dim: int, n_pos: int, device="cuda", ctx: Context | None = None):
@@ -194,7 +208,8 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, kv_lens, scale: float, w
     else:
         os = _rows(out, "out", n_seqs, hq, d, dev, dt)
     h = _bind(ctx, dev)
-    ws, n = _workspace((dev, code, hkv, hq, d), q, _lib.sa_attn_paged_decode_workspace, h, kv, hq)
+    n = _size((dev, code, hkv, hq, d), _lib.sa_attn_paged_decode_workspace, h, kv, hq)
+    ws = _decode_workspace(dev, n)
     check(_lib.sa_attn_paged_decode(h, kv, q.data_ptr(), qs, hq, window, sinks, scale, out.data_ptr(), os, ws.data_ptr(), n))
     return out
 
@@ -243,8 +258,8 @@ def attn_paged_decode_prefix(q, k_pages, v_pages, prefix_table, prefix_len: int,
     else:
         os = _rows(out, "out", n_seqs, hq, d, dev, dt)
     h = _bind(ctx, dev)
-    ws, n = _workspace((dev, code, hkv, hq, d, n_seqs, prefix_len), q, _lib.sa_attn_paged_decode_prefix_workspace, h, kv, hq,
-                       prefix_len)
+    n = _size((dev, code, hkv, hq, d, n_seqs, prefix_len), _lib.sa_attn_paged_decode_prefix_workspace, h, kv, hq, prefix_len)
+    ws = q.new_empty(-(-n // q.element_size()))
     check(_lib.sa_attn_paged_decode_prefix(h, kv, pp, prefix_len, q.data_ptr(), qs, hq, scale, out.data_ptr(), os,
                                            ws.data_ptr(), n))
     return out
