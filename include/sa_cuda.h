@@ -378,10 +378,10 @@ int sa_attn_decode_noalloc(void* stream, int dtype, const void* q, const void* k
  *
  * Workspaces are the caller's (256-byte aligned device memory); calls that may
  * run at the same time, captured ones included, need workspaces of their own.
- * Their sizes depend on the shapes in kv and on hq, not on lengths.  The first
- * SA_PAGED_ZERO_BYTES of that of sa_attn_paged_decode are zeros before its first
- * use; every call, of any shape, leaves them zero for the next.  All else may
- * hold anything.  out may be q.
+ * Their sizes depend on the shapes in kv, on hq and on the prefix's length, not
+ * on the sequences'.  A workspace's first SA_PAGED_ZERO_BYTES are zeros before
+ * its first use, and every call, of either kind and any shape, leaves them zero
+ * for the next; all else may hold anything.  out may be q.
  */
 #define SA_PAGED_MAX_SEQS 65536
 #define SA_PAGED_ZERO_BYTES 4096

@@ -44,6 +44,7 @@ namespace pg {
 constexpr int STAGES = 3;
 constexpr float LOG2E = 1.4426950408889634f;
 
+enum { JOIN_HERE = 1, JOIN_LATER = 2 };
 struct DecodeArgs {
     Cache c;
     const void* q;
@@ -51,7 +52,8 @@ struct DecodeArgs {
     long long q_stride, o_stride;      // elements between sequences
     int hq, G, window, sinks;
     float qscale;                      // scale * log2(e)
-    int to_state;                      // 1: leave every state in `st` (a shared prefix is joined later)
+    int prefixed;                      // every query sees a shared prefix too; JOIN_HERE or JOIN_LATER
+    PrefixParts prefix;
     DecodeWs ws;
 };
 
@@ -62,6 +64,14 @@ struct Geo {
     static constexpr int TK = STAGE_BYTES / (2 * D * ELT);                          // rows of a tile
     static constexpr int CTAS = STAGE_BYTES == 32768 ? 2 : 1;                       // per SM
 };
+
+// The tiles of a sequence's own rows.  Where a prefix's parts are joined here, a
+// sequence without own rows has an empty one, so that somebody does it.
+__device__ __forceinline__ Tiles tiles_of(const DecodeArgs& a, int len, int tk) {
+    Tiles t = make_tiles(len, a.window, a.sinks, tk);
+    if (a.prefixed == JOIN_HERE && t.n == 0) t.n = 1;
+    return t;
+}
 
 // This CTA's share of the tile list, and the walk through it.
 struct Walk {
@@ -77,7 +87,7 @@ struct Walk {
         if (!left) return;
         do {
             ++b;
-            t = make_tiles(seq_len(a.c, b), a.window, a.sinks, tk);
+            t = tiles_of(a, seq_len(a.c, b), tk);
         } while (t.n == 0);
     }
 };
@@ -104,7 +114,7 @@ __device__ void plan_share(const DecodeArgs& a, int tk, Share* s, long long* sca
         for (int u = 0; u < 8; ++u) len[u] = b + u < b1 ? a.c.kv_lens[b + u] : 0;
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            mine += make_tiles(cut_len(len[u], a.c.max_pages, a.c.page_log2), a.window, a.sinks, tk).n;
+            if (b + u < b1) mine += tiles_of(a, cut_len(len[u], a.c.max_pages, a.c.page_log2), tk).n;
     }
     mine *= a.c.hkv;
     long long inc = mine;
@@ -131,7 +141,7 @@ __device__ void plan_share(const DecodeArgs& a, int tk, Share* s, long long* sca
             if (f >= start && f < start + mine) {
                 long long at = start;
                 for (int b = b0; b < b1; ++b) {
-                    const int nt = make_tiles(seq_len(a.c, b), a.window, a.sinks, tk).n;
+                    const int nt = tiles_of(a, seq_len(a.c, b), tk).n;
                     const long long all = (long long)nt * a.c.hkv;
                     if (f < at + all) {
                         s->b = b;
@@ -148,9 +158,8 @@ __device__ void plan_share(const DecodeArgs& a, int tk, Share* s, long long* sca
             }
         }
     }
-    // sequences without a visible row: their output is zero (their state, where
-    // a prefix follows, is read from nobody: the join looks at the length)
-    if (!a.to_state)
+    // sequences without a visible row: their output is zero
+    if (!a.prefixed)
         for (int b = b0; b < b1; ++b) {
             if (b % gridDim.x != blockIdx.x || seq_len(a.c, b) > 0) continue;
             const int e = a.ws.out_elt;
@@ -161,8 +170,8 @@ __device__ void plan_share(const DecodeArgs& a, int tk, Share* s, long long* sca
     __syncthreads();
 }
 
-// Where a pair's state goes: straight to the output, to the pair's own state
-// (a prefix follows), or to a slot of this CTA that the join reads.
+// Where a pair's state goes: straight to the output, to the pair's own state (to
+// be joined with a prefix's parts), or to a slot of this CTA.
 enum { TO_OUT = 0, TO_STATE = 1, TO_SLOT = 2 };
 struct Dest {
     int kind, slot;
@@ -171,7 +180,7 @@ struct Dest {
 __device__ __forceinline__ Dest segment_dest(const DecodeArgs& a, const Share& s, long long seg_first, bool whole,
                                              int b, int h) {
     Dest d;
-    d.kind = !whole ? TO_SLOT : a.to_state ? TO_STATE : TO_OUT;
+    d.kind = !whole ? TO_SLOT : a.prefixed ? TO_STATE : TO_OUT;
     d.slot = whole ? b * a.c.hkv + h : 2 * (int)blockIdx.x + (seg_first == s.first ? 0 : 1);
     return d;
 }
@@ -234,7 +243,7 @@ __device__ __forceinline__ bool consume_wait(Ring* r, int it, bool& ok, int* sta
     return false;
 }
 
-// With a prefix to come: where the join finds a pair's state.
+// For a kernel that joins the states later: where it finds a pair's.
 __device__ __forceinline__ void record_pair(const DecodeArgs& a, const Share& s, long long t0, int n, int i0, bool whole,
                                             int b, int h) {
     const int pair = b * a.c.hkv + h;
@@ -246,24 +255,40 @@ __device__ __forceinline__ void record_pair(const DecodeArgs& a, const Share& s,
     }
 }
 
-// The consumer threads have written a share's state (thread 0's warp did): count
-// it, and where it was the pair's last, join the pair: a warp per query head.
+// The consumer threads have written the state of a pair, or of a share of one
+// (thread 0's warp did).  Count a share; then join what there is to join -- the
+// prefix's parts, the pair's shares where this was the last one handed in -- with
+// a warp per query head.
 template <typename OT, int D, int NT>
-__device__ __forceinline__ void hand_in(const DecodeArgs& a, Ring* r, const Share& sh, long long t0, int n, int b, int h) {
+__device__ __forceinline__ void hand_in(const DecodeArgs& a, Ring* r, const Share& sh, long long t0, int n, bool whole,
+                                        int b, int h) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const Shares x = pair_shares(sh, t0, n);
-    const int parts = x.last - x.first + 1;
+    Shares x = {};
+    int shares = 1;
     __threadfence();
     bar_consumers<NT>();
-    if (threadIdx.x == 0) r->last = atomicAdd(a.ws.count + x.first, 1u) == (unsigned)(parts - 1);
-    bar_consumers<NT>();
-    if (!r->last) return;
-    __threadfence();
-    if (threadIdx.x == 0) a.ws.count[x.first] = 0u;
+    if (!whole) {
+        x = pair_shares(sh, t0, n);
+        shares = x.last - x.first + 1;
+        if (threadIdx.x == 0) r->last = atomicAdd(a.ws.count + x.first, 1u) == (unsigned)(shares - 1);
+        bar_consumers<NT>();
+        if (!r->last) return;
+        __threadfence();
+        if (threadIdx.x == 0) a.ws.count[x.first] = 0u;
+    }
+    if (a.prefixed) pdl_wait();
+    const long long rows = (long long)a.c.n_seqs * a.hq;
     for (int g = warp; g < a.G; g += NT / 32) {
+        const long long row = (long long)b * a.hq + h * a.G + g;
         Joined<D> s;
-        s.add(parts, lane, [&](int p) { return __ldcg(a.ws.slot_ml + share_slot(x, p) * a.G + g); },
-              [&](int p) { return a.ws.slot_o + (share_slot(x, p) * a.G + g) * D; });
+        if (a.prefixed)
+            s.add(a.prefix.parts, lane, [&](int p) { return __ldcg(a.prefix.ml + p * rows + row); },
+                  [&](int p) { return a.prefix.o + (p * rows + row) * D; });
+        if (whole)
+            s.add(1, lane, [&](int) { return __ldcg(a.ws.state_ml + row); }, [&](int) { return a.ws.state_o + row * D; });
+        else
+            s.add(shares, lane, [&](int p) { return __ldcg(a.ws.slot_ml + share_slot(x, p) * a.G + g); },
+                  [&](int p) { return a.ws.slot_o + (share_slot(x, p) * a.G + g) * D; });
         s.store(static_cast<OT*>(a.out) + (long long)b * a.o_stride + (long long)(h * a.G + g) * D, lane);
     }
 }
@@ -338,11 +363,10 @@ __device__ __forceinline__ void drain(Ring* r) {
     __syncthreads();
 }
 
-// Behind a shared prefix the launch starts while the prefix's kernel still runs
-// (neither reads what the other writes); it ends only after that kernel, so that
-// the join, which waits for this one, has both.
+// Behind a shared prefix the launch starts while the prefix's kernel still runs;
+// it ends only after that kernel, so that the stream's next one has both.
 __device__ __forceinline__ void leave(const DecodeArgs& a) {
-    if (a.to_state) pdl_wait();                          // (nothing to wait for in an ordinary launch)
+    if (a.prefixed) pdl_wait();                          // (nothing to wait for in an ordinary launch)
 }
 
 // ---- bf16 -------------------------------------------------------------------
@@ -416,7 +440,7 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     if (tid == 0) r.consumed = sh.count;
     Walk w;
     w.b = sh.b; w.h = sh.h; w.i = sh.i; w.left = sh.count;
-    w.t = make_tiles(seq_len(a.c, w.b), a.window, a.sinks, TK);
+    w.t = tiles_of(a, seq_len(a.c, w.b), TK);
     __syncthreads();
 
     if (warp == BW) {
@@ -608,10 +632,10 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 }
             }
         }
-        if (a.to_state) {
+        if (a.prefixed == JOIN_LATER) {
             if (tid == 0) record_pair(a, sh, seg_first - i0, t.n, i0, whole, b, h);
-        } else if (!whole) {
-            hand_in<__nv_bfloat16, D, BW * 32>(a, &r, sh, seg_first - i0, t.n, b, h);
+        } else if (a.prefixed || !whole) {
+            hand_in<__nv_bfloat16, D, BW * 32>(a, &r, sh, seg_first - i0, t.n, whole, b, h);
         }
     }
     drain(&r);
@@ -663,7 +687,7 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
     if (tid == 0) r.consumed = sh.count;
     Walk w;
     w.b = sh.b; w.h = sh.h; w.i = sh.i; w.left = sh.count;
-    w.t = make_tiles(seq_len(a.c, w.b), a.window, a.sinks, TK);
+    w.t = tiles_of(a, seq_len(a.c, w.b), TK);
     __syncthreads();
 
     if (warp == NW) {
@@ -841,10 +865,10 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
                 if (col == 0) (ds.kind == TO_STATE ? a.ws.state_ml : a.ws.slot_ml)[at] = make_float2(M, L);
             }
         }
-        if (a.to_state) {
+        if (a.prefixed == JOIN_LATER) {
             if (tid == 0) record_pair(a, sh, seg_first - i0, t.n, i0, whole, b, h);
-        } else if (!whole) {
-            hand_in<float, D, NW * 32>(a, &r, sh, seg_first - i0, t.n, b, h);
+        } else if (a.prefixed || !whole) {
+            hand_in<float, D, NW * 32>(a, &r, sh, seg_first - i0, t.n, whole, b, h);
         }
         bar_consumers<NW * 32>();                        // the buffers are free again
     }
@@ -902,8 +926,8 @@ static int launch_bf16(cudaStream_t st, int grid, bool overlap, const CUtensorMa
 }
 
 int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_stride, int hq, int window, int sinks,
-                  float scale, void* out, long long o_stride, bool to_state, bool overlap, const DecodeWs& ws) {
-    DecodeArgs a;
+                  float scale, void* out, long long o_stride, const PrefixParts* prefix, const DecodeWs& ws) {
+    DecodeArgs a = {};
     a.c = make_cache(ctx, kv);
     a.q = q;
     a.out = out;
@@ -914,8 +938,10 @@ int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q
     a.window = window;
     a.sinks = sinks;
     a.qscale = scale * LOG2E;
-    a.to_state = to_state ? 1 : 0;
+    a.prefixed = !prefix ? 0 : prefix->join ? JOIN_HERE : JOIN_LATER;
+    if (prefix) a.prefix = *prefix;
     a.ws = ws;
+    const bool overlap = prefix && prefix->parts > 0;
     const int grid = decode_grid(ctx, kv, hq);
     cudaStream_t st = ctx->stream;
     if (kv->dtype == SA_F32) {
@@ -927,21 +953,20 @@ int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q
             p.fn<<<grid, p.threads, p.smem, st>>>(a);
             SA_CUDA_TRY(cudaGetLastError());
         }
-    } else {
-        CUtensorMap tk, tv;
-        const int tile = kv->d == 64 ? Geo<__nv_bfloat16, 64>::TK : Geo<__nv_bfloat16, 128>::TK;
-        const int box = std::min(kv->page_size, tile);
-        SA_RC_TRY(make_page_tmap(&tk, kv->k_pages, kv, box));
-        SA_RC_TRY(make_page_tmap(&tv, kv->v_pages, kv, box));
-        SA_RC_TRY(kv->d == 64    ? launch_bf16<64>(st, grid, overlap, tk, tv, a)
-                  : kv->d == 128 ? launch_bf16<128>(st, grid, overlap, tk, tv, a)
-                                 : launch_bf16<256>(st, grid, overlap, tk, tv, a));
+        return SA_OK;
     }
-    return SA_OK;
+    CUtensorMap tk, tv;
+    const int tile = kv->d == 64 ? Geo<__nv_bfloat16, 64>::TK : Geo<__nv_bfloat16, 128>::TK;
+    const int box = std::min(kv->page_size, tile);
+    SA_RC_TRY(make_page_tmap(&tk, kv->k_pages, kv, box));
+    SA_RC_TRY(make_page_tmap(&tv, kv->v_pages, kv, box));
+    return kv->d == 64    ? launch_bf16<64>(st, grid, overlap, tk, tv, a)
+           : kv->d == 128 ? launch_bf16<128>(st, grid, overlap, tk, tv, a)
+                          : launch_bf16<256>(st, grid, overlap, tk, tv, a);
 }
 
-size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool to_state, void* base, DecodeWs* ws) {
-    const int grid = decode_grid(ctx, kv, hq), G = hq / kv->hkv;      // grid <= SA_PAGED_ZERO_BYTES / 4
+size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool prefix, void* base, DecodeWs* ws) {
+    const int grid = decode_grid(ctx, kv, hq), G = hq / kv->hkv;
     const size_t slots = (size_t)grid * 2 * G, rows = (size_t)kv->n_seqs * hq, d4 = (size_t)kv->d * 4;
     size_t at = 0;
     unsigned char* p = static_cast<unsigned char*>(base);
@@ -952,13 +977,13 @@ size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool t
     };
     DecodeWs w = {};
     // first, and as long for every shape: calls of other shapes leave it zero too
-    if (!to_state) w.count = reinterpret_cast<unsigned*>(take(SA_PAGED_ZERO_BYTES));
+    w.count = reinterpret_cast<unsigned*>(take(SA_PAGED_ZERO_BYTES));
     w.slot_o = reinterpret_cast<float*>(take(slots * d4));
     w.slot_ml = reinterpret_cast<float2*>(take(slots * 8));
-    if (to_state) {
-        w.pair = reinterpret_cast<int4*>(take((size_t)kv->n_seqs * kv->hkv * sizeof(int4)));
+    if (prefix) {
         w.state_o = reinterpret_cast<float*>(take(rows * d4));
         w.state_ml = reinterpret_cast<float2*>(take(rows * 8));
+        w.pair = reinterpret_cast<int4*>(take((size_t)kv->n_seqs * kv->hkv * sizeof(int4)));
     }
     w.d = kv->d;
     w.out_elt = kv->dtype == SA_F32 ? 4 : 2;
@@ -1000,5 +1025,5 @@ SA_API int sa_attn_paged_decode(sa_ctx* ctx, const sa_paged_kv* kv, const void* 
     const size_t need = pg::decode_ws_layout(ctx, kv, hq, false, workspace, &ws);
     SA_CHECK_ARG(workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need,
                  "%s: workspace of %zu bytes (want %zu, 256-byte aligned)", fn, workspace_bytes, need);
-    return pg::decode_launch(ctx, kv, q, q_stride, hq, window, sinks, scale, out, o_stride, false, false, ws);
+    return pg::decode_launch(ctx, kv, q, q_stride, hq, window, sinks, scale, out, o_stride, nullptr, ws);
 }

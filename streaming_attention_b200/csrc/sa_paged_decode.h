@@ -6,27 +6,36 @@
 namespace sa {
 namespace pg {
 
-// Shares of (sequence, KV head) pairs that several CTAs hold: unnormalised O
-// rows of d floats and (m in the log2 domain, l).
+// States of (sequence, KV head) pairs: unnormalised O rows of d floats, and
+// (m in the log2 domain, l).
 struct DecodeWs {
-    float* slot_o;    // [grid][2][G][d]: the first and the last pair of a CTA
+    unsigned* count;  // [SA_PAGED_ZERO_BYTES / 4]: shares handed in of the pair whose first one CTA i holds; zero
+                      // between calls
+    float* slot_o;    // [grid][2][G][d]: shares of pairs that several CTAs hold, each CTA's first and last pair
     float2* slot_ml;  // [grid][2][G]
-    unsigned* count;  // [grid]: shares handed in of the pair whose first one the CTA holds; zero between calls
-    int4* pair;       // [n_seqs * hkv]: first CTA (-1: the state is whole), last CTA, first CTA's slot; with `state`
-    float* state_o;   // [n_seqs][hq][d]
+    float* state_o;   // [n_seqs][hq][d]: whole pairs, where a prefix's parts are to be joined with them
     float2* state_ml; // [n_seqs][hq]
+    int4* pair;       // [n_seqs * hkv]: where a pair's state is: its first CTA (-1: whole), last CTA, first one's slot
     int d, out_elt;
+};
+// What a shared prefix left: states of every query row, [parts][n_seqs * hq].
+struct PrefixParts {
+    const float* o;
+    const float2* ml;
+    int parts;
+    bool join;        // false: the launch leaves the pairs' states for a kernel that joins them with the parts
 };
 
 int decode_grid(const sa_ctx* ctx, const sa_paged_kv* kv, int hq);
-// Lays the workspace out at `base` (may be null) and returns its size.
-size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool to_state, void* base, DecodeWs* ws);
-// to_state: every pair's state goes to ws (pair, state, slots) and `out` is not
-// written.  overlap: the stream's last kernel is a shared prefix's, which started
-// after everything that this launch reads was written; the launch may start while
-// it runs.
+// Lays the workspace out at `base` (may be null) and returns its size; prefix:
+// with room for whole pairs' states.
+size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool prefix, void* base, DecodeWs* ws);
+// prefix (may be null): the rows of a shared prefix come before each sequence's
+// own.  Where it has parts, the stream's last kernel is the one that computes
+// them, which started after everything else that this launch reads was written:
+// the launch may start while it runs, and waits for it before it joins.
 int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_stride, int hq, int window, int sinks,
-                  float scale, void* out, long long o_stride, bool to_state, bool overlap, const DecodeWs& ws);
+                  float scale, void* out, long long o_stride, const PrefixParts* prefix, const DecodeWs& ws);
 
 }  // namespace pg
 }  // namespace sa

@@ -1,14 +1,14 @@
 // sa_paged_prefix.cu -- the C entries of the paged prefill and of the decode
-// behind a shared prefix, and the join of the latter's states.
+// behind a shared prefix.
 //
-// softmax over [prefix rows, own rows] from states (m, l, O) of parts of them:
+// The latter's softmax over [prefix rows, own rows] comes from states (m, l, O) of
+// parts of them:
 //   m = max m_i,  l = sum 2^(m_i - m) l_i,  O = sum 2^(m_i - m) O_i,  out = O / l.
 // The prefix is read once for all sequences: its query rows are the B x G
 // (sequence, head) pairs of a KV head, a matrix product with B G rows where a
-// decode per sequence would read the prefix B times.
-#include <cuda_bf16.h>
-#include <algorithm>
-
+// decode per sequence would read the prefix B times.  The decode over the
+// sequences' own rows starts while that product's last CTAs run, and joins its
+// parts with its own states.
 #include "sa_paged.cuh"
 #include "sa_paged_decode.h"
 #include "sa_paged_f32.h"
@@ -155,15 +155,31 @@ SA_API int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const
     SA_RC_TRY(check_prefix(fn, kv, hq, prefix_table, prefix_len));
     SA_RC_TRY(pg::check_scale(fn, scale));
     if (kv->n_seqs == 0) return SA_OK;
-    const int e = kv->dtype == SA_F32 ? 4 : 2, d = kv->d;
-    SA_RC_TRY(pg::check_rows(fn, "q", q, q_stride, (long long)hq * d, e));
-    SA_RC_TRY(pg::check_rows(fn, "out", out, o_stride, (long long)hq * d, e));
+    const int e = kv->dtype == SA_F32 ? 4 : 2;
+    SA_RC_TRY(pg::check_rows(fn, "q", q, q_stride, (long long)hq * kv->d, e));
+    SA_RC_TRY(pg::check_rows(fn, "out", out, o_stride, (long long)hq * kv->d, e));
     SA_CHECK_ARG(ctx != nullptr, "%s: ctx is NULL", fn);
     DeviceGuard guard(ctx->device);
     pg::PrefixWs ws;
     const size_t need = pg::prefix_ws_layout(ctx, kv, hq, prefix_len, workspace, &ws);
     SA_CHECK_ARG(workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need,
                  "%s: workspace of %zu bytes (want %zu, 256-byte aligned)", fn, workspace_bytes, need);
+    if (prefix_len > 0) {
+        if (kv->dtype == SA_F32)
+            SA_RC_TRY(pg::f32_prefix_launch(ctx, kv, static_cast<const float*>(q), q_stride, hq, prefix_table,
+                                            prefix_len, scale, ws.n_split, ws.part_o, ws.part_ml));
+        else
+            SA_RC_TRY(pg::tc_prefix_launch(ctx, kv, q, q_stride, hq, prefix_table, prefix_len, scale, ws.n_split,
+                                           ws.part_o, ws.part_ml));
+    }
+    // Few pairs and parts: the decode's CTAs join the parts themselves.  Else a kernel
+    // of its own does, with four warps per row where a CTA of the decode has one
+    // (16/8 heads, 8 sequences behind 1000 rows: 13.1 us here, 14.9 there; 16 behind
+    // 4000: 24.8 and 22.5).
+    const bool join = kv->n_seqs * kv->hkv <= 64 && ws.parts <= 16;
+    const pg::PrefixParts parts = {ws.part_o, reinterpret_cast<const float2*>(ws.part_ml), ws.parts, join};
+    SA_RC_TRY(pg::decode_launch(ctx, kv, q, q_stride, hq, 0, 0, scale, out, o_stride, &parts, ws.own));
+    if (join) return SA_OK;
     pg::JoinArgs j;
     j.c = pg::make_cache(ctx, kv);
     j.ws = ws.own;
@@ -174,20 +190,10 @@ SA_API int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const
     j.parts = ws.parts;
     j.part_o = ws.part_o;
     j.part_ml = ws.part_ml;
-    if (prefix_len > 0) {
-        if (kv->dtype == SA_F32) {
-            SA_RC_TRY(pg::f32_prefix_launch(ctx, kv, static_cast<const float*>(q), q_stride, hq, prefix_table,
-                                            prefix_len, scale, ws.n_split, ws.part_o, ws.part_ml));
-        } else {
-            SA_RC_TRY(pg::tc_prefix_launch(ctx, kv, q, q_stride, hq, prefix_table, prefix_len, scale, ws.n_split,
-                                           ws.part_o, ws.part_ml));
-        }
-    }
-    SA_RC_TRY(pg::decode_launch(ctx, kv, q, q_stride, hq, 0, 0, scale, nullptr, 0, true, prefix_len > 0, ws.own));
     const dim3 grid((unsigned)(kv->n_seqs * (long long)hq));
-    auto k = kv->dtype == SA_F32 ? (d == 64 ? pg::prefix_join_kernel<float, 64> : pg::prefix_join_kernel<float, 128>)
-                                 : (d == 64 ? pg::prefix_join_kernel<__nv_bfloat16, 64>
-                                            : pg::prefix_join_kernel<__nv_bfloat16, 128>);
+    auto k = kv->dtype == SA_F32
+                 ? (kv->d == 64 ? pg::prefix_join_kernel<float, 64> : pg::prefix_join_kernel<float, 128>)
+                 : (kv->d == 64 ? pg::prefix_join_kernel<__nv_bfloat16, 64> : pg::prefix_join_kernel<__nv_bfloat16, 128>);
     SA_CUDA_TRY(launch_pdl(k, grid, dim3(pg::JT), 0, ctx->stream, j));
     return SA_OK;
 }

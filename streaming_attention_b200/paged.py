@@ -31,7 +31,7 @@ from ._capi import SA_BF16, SA_F32, SA_PAGED_ZERO_BYTES, Context, check, default
 _torch = None
 _lib = None
 _sizes: dict = {}
-_decode_ws: dict = {}
+_kept: dict = {}
 # the members of sa_paged_kv in order, natively aligned
 _pack = struct.Struct("@PPiiiiiqPqiPi").pack
 
@@ -125,16 +125,16 @@ def _size(key, size_fn, *args) -> int:
     return n
 
 
-def _decode_workspace(dev: int, n: int):
-    """The decode's workspace, its head zero: kept from call to call of a stream; a captured call has its own."""
+def _workspace(dev: int, n: int):
+    """A decode's workspace, its head zero: kept from call to call of a stream; a captured call has its own."""
     if _torch._C._cuda_isCurrentStreamCapturing():
         ws = _torch.empty(n, dtype=_torch.uint8, device=dev)
         ws[:SA_PAGED_ZERO_BYTES].zero_()
         return ws
     key = (dev, _torch._C._cuda_getCurrentRawStream(dev))
-    ws = _decode_ws.get(key)
+    ws = _kept.get(key)
     if ws is None or ws.numel() < n:
-        ws = _decode_ws[key] = _torch.zeros(n, dtype=_torch.uint8, device=dev)
+        ws = _kept[key] = _torch.zeros(n, dtype=_torch.uint8, device=dev)
     return ws
 
 
@@ -209,7 +209,7 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, kv_lens, scale: float, w
         os = _rows(out, "out", n_seqs, hq, d, dev, dt)
     h = _bind(ctx, dev)
     n = _size((dev, code, hkv, hq, d), _lib.sa_attn_paged_decode_workspace, h, kv, hq)
-    ws = _decode_workspace(dev, n)
+    ws = _workspace(dev, n)
     check(_lib.sa_attn_paged_decode(h, kv, q.data_ptr(), qs, hq, window, sinks, scale, out.data_ptr(), os, ws.data_ptr(), n))
     return out
 
@@ -259,7 +259,7 @@ def attn_paged_decode_prefix(q, k_pages, v_pages, prefix_table, prefix_len: int,
         os = _rows(out, "out", n_seqs, hq, d, dev, dt)
     h = _bind(ctx, dev)
     n = _size((dev, code, hkv, hq, d, n_seqs, prefix_len), _lib.sa_attn_paged_decode_prefix_workspace, h, kv, hq, prefix_len)
-    ws = q.new_empty(-(-n // q.element_size()))
+    ws = _workspace(dev, n)
     check(_lib.sa_attn_paged_decode_prefix(h, kv, pp, prefix_len, q.data_ptr(), qs, hq, scale, out.data_ptr(), os,
                                            ws.data_ptr(), n))
     return out
