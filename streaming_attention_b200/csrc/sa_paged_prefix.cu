@@ -30,16 +30,17 @@ struct JoinArgs {
     const float* part_ml;
 };
 
-// Four warps per (sequence, query head): a quarter of the prefix's parts each,
-// the last one the sequence's own rows too.
-template <typename OT, int D>
+// W warps per (sequence, query head): a share of the prefix's parts each, the last
+// one the sequence's own rows too.
+template <typename OT, int D, int W>
 __global__ void __launch_bounds__(JT) prefix_join_kernel(const __grid_constant__ JoinArgs a) {
-    constexpr int W = JT / 32, V = D / 32;
-    __shared__ float s_o[W - 1][D];
-    __shared__ float2 s_ml[W - 1];
+    constexpr int V = D / 32, R = JT / 32 / W;             // rows of a CTA
+    __shared__ float s_o[R][W][D];
+    __shared__ float2 s_ml[R][W];
     pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long row = blockIdx.x, rows = (long long)a.c.n_seqs * a.hq;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % W, r = (threadIdx.x >> 5) / W;
+    const long long row = (long long)blockIdx.x * R + r, rows = (long long)a.c.n_seqs * a.hq;
+    if (W == 1 && row >= rows) return;                     // R = 1 otherwise: no such row
     const int b = (int)(row / a.hq), h = (int)(row - (long long)b * a.hq), kvh = h / a.G, g = h - kvh * a.G;
     const int p0 = warp * a.parts / W, p1 = (warp + 1) * a.parts / W;
     Joined<D> s;
@@ -55,17 +56,29 @@ __global__ void __launch_bounds__(JT) prefix_join_kernel(const __grid_constant__
                   [&](int p) { return a.ws.slot_o + at(p) * D; });
         }
     }
-    if (warp > 0) {
-        const float l = s.total();
-        if (lane == 0) s_ml[warp - 1] = make_float2(s.m, l);
+    if constexpr (W > 1) {
+        if (warp > 0) {
+            const float l = s.total();
+            if (lane == 0) s_ml[r][warp] = make_float2(s.m, l);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s_o[warp - 1][lane * V + e] = s.o[e];
+            for (int e = 0; e < V; ++e) s_o[r][warp][lane * V + e] = s.o[e];
+        }
+        __syncthreads();
+        if (warp > 0) return;
+#pragma unroll
+        for (int w = 1; w < W; ++w) s.add_one(lane, s_ml[r][w].x, s_ml[r][w].y, s_o[r][w]);
     }
-    __syncthreads();
-    if (warp > 0) return;
-#pragma unroll
-    for (int w = 0; w < W - 1; ++w) s.add_one(lane, s_ml[w].x, s_ml[w].y, s_o[w]);
     s.store(static_cast<OT*>(a.out) + (long long)b * a.o_stride + (long long)h * D, lane);
+}
+
+template <typename OT, int D>
+static int join_launch(const sa_ctx* ctx, const JoinArgs& j) {
+    const long long rows = (long long)j.c.n_seqs * j.hq;
+    if (rows < 8LL * ctx->num_sms)
+        SA_CUDA_TRY(launch_pdl(prefix_join_kernel<OT, D, 4>, dim3((unsigned)rows), dim3(JT), 0, ctx->stream, j));
+    else
+        SA_CUDA_TRY(launch_pdl(prefix_join_kernel<OT, D, 1>, dim3((unsigned)((rows + 3) / 4)), dim3(JT), 0, ctx->stream, j));
+    return SA_OK;
 }
 
 struct PrefixWs {
@@ -173,9 +186,10 @@ SA_API int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const
                                            ws.part_o, ws.part_ml));
     }
     // Few pairs and parts: the decode's CTAs join the parts themselves.  Else a kernel
-    // of its own does, with four warps per row where a CTA of the decode has one
-    // (16/8 heads, 8 sequences behind 1000 rows: 13.1 us here, 14.9 there; 16 behind
-    // 4000: 24.8 and 22.5).
+    // of its own does (16/8 heads, 8 sequences behind 1000 rows: 13.1 us here, 14.9
+    // there; 16 behind 4000: 24.8 and 22.5), with four warps per row where the rows
+    // would not fill the GPU (256 rows of 37 parts: 10.0 us, with one warp each 13.0;
+    // 2048 rows of 18 parts: 16.0 and 10.6).
     const bool join = kv->n_seqs * kv->hkv <= 64 && ws.parts <= 16;
     const pg::PrefixParts parts = {ws.part_o, reinterpret_cast<const float2*>(ws.part_ml), ws.parts, join};
     SA_RC_TRY(pg::decode_launch(ctx, kv, q, q_stride, hq, 0, 0, scale, out, o_stride, &parts, ws.own));
@@ -190,10 +204,7 @@ SA_API int sa_attn_paged_decode_prefix(sa_ctx* ctx, const sa_paged_kv* kv, const
     j.parts = ws.parts;
     j.part_o = ws.part_o;
     j.part_ml = ws.part_ml;
-    const dim3 grid((unsigned)(kv->n_seqs * (long long)hq));
-    auto k = kv->dtype == SA_F32
-                 ? (kv->d == 64 ? pg::prefix_join_kernel<float, 64> : pg::prefix_join_kernel<float, 128>)
-                 : (kv->d == 64 ? pg::prefix_join_kernel<__nv_bfloat16, 64> : pg::prefix_join_kernel<__nv_bfloat16, 128>);
-    SA_CUDA_TRY(launch_pdl(k, grid, dim3(pg::JT), 0, ctx->stream, j));
-    return SA_OK;
+    return kv->dtype == SA_F32 ? (kv->d == 64 ? pg::join_launch<float, 64>(ctx, j) : pg::join_launch<float, 128>(ctx, j))
+                               : (kv->d == 64 ? pg::join_launch<__nv_bfloat16, 64>(ctx, j)
+                                              : pg::join_launch<__nv_bfloat16, 128>(ctx, j));
 }
