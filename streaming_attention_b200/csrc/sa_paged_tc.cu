@@ -31,6 +31,14 @@
 //  * rows behind the sequence's last one share a page with it and may hold
 //    anything: K's are masked, V's are overwritten with zeros in shared memory
 //    by the softmax threads before the tile's P is handed over.
+//
+// Bound: the tensor pipe and the exponentials, each busy 56% of the time.
+// Measured (16/8 heads of 128, short bursts): 8192 tokens under a window of 4096
+// 182 us, 1130 TFLOP/s of visible work, 0.67 of the measured bf16 peak; 512 tokens
+// over 1100 visible rows 19 us; the prefix part of 64 sequences (32/8 heads) behind
+// 32768 rows 40 us, 0.86 PFLOP/s.  A tile of two slots takes some 3150 clocks, of
+// which the tensor core works 2048 and a slot's exponentials 1400: with S, P and O
+// of two slots TMEM is full, and a slot's S waits for its P.V.
 #include <algorithm>
 #include <cmath>
 
