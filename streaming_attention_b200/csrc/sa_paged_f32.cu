@@ -12,17 +12,20 @@
 // pairs would run twice as fast, at 2^-17.)
 //
 // A CTA of eight warps holds FM query rows (FM / G tokens times the G heads of a
-// KV head) and walks over tiles of 64 keys: S = Q K^T with 16 rows per warp, the
-// warps of a row group sharing the keys; the row maximum and P through shared
-// memory; O += P V with the row group's warps sharing O's columns.  K and V of the
-// next tile are copied (cp.async) as soon as their buffers are free: K under the
-// softmax and P V, V under the next S.  Rows that no query of the CTA sees are
-// not read but zero-filled.
+// KV head) and walks over tiles of 64 keys: S = Q K^T with 16 rows per warp (32 at
+// FM = 128: an operand is split once for twice the products), the warps of a row
+// group sharing the keys; the row maximum and P through shared memory; O += P V with
+// the row group's warps sharing O's columns.  K and V of the next tile are copied
+// (cp.async) as soon as their buffers are free: K under the softmax and P V, V under
+// the next S; the page of the tile after it is looked up meanwhile.  Rows that no
+// query of the CTA sees are not read but zero-filled.
 //
-// Bound: the tensor pipe (0.35 busy) and the latency of few dependent tiles.
+// Bound: the tensor pipe (0.60 busy over 4096 causal tokens) with the splits and the
+// softmax between its products; small calls by the latency of few dependent tiles.
 // Measured: 16 sequences behind 4001 rows, 16/8 heads of 128: 22.9 us for the
 // prefix (42 on FMAs); three chunks of up to 300 tokens, 8/4 heads of 64, window
-// 129: 21.9 us (29); errors against 64 bits 2e-7.
+// 129: 21.8 us (29); 4096 tokens, 16/8 heads of 128: 1260 us, 55 TFLOP/s of 97 (45
+// with 64 rows); errors against 64 bits 2e-7.
 #include <algorithm>
 #include <cmath>
 
@@ -53,7 +56,8 @@ struct FLay {
     // Row strides of 4 mod 32 words: the eight rows of an ldmatrix, and the V
     // elements of a fragment (rows two apart, eight columns), hit all banks.
     static constexpr int RS = D + 4, PS = FN + 4;
-    static constexpr int WM = FM / 16, WN = 8 / WM;    // warps over rows; over keys, then over columns
+    static constexpr int MR = FM == 128 ? 2 : 1;       // 16-row blocks per warp
+    static constexpr int WM = FM / 16 / MR, WN = 8 / WM;    // warps over rows; over keys, then over columns
     static constexpr int Q = 0, K = FM * RS, V = K + FN * RS, P = V + FN * RS, X = P + FM * PS;
     static constexpr int SMEM = (X + WN * FM) * 4;
 };
@@ -67,16 +71,42 @@ __device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// c += A B of one step: the tensor core cuts its sums off where fp32 rounds, so
-// it sums eight products from zero and the long sum is an fp32 addition.
-__device__ __forceinline__ void mma_exact(float (&c)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t bh0,
-                                          uint32_t bh1, uint32_t bl0, uint32_t bl1) {
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
-    mma1688(d, al, bh0, bh1);
-    mma1688(d, ah, bl0, bl1);
-    mma1688(d, ah, bh0, bh1);
+// The product's first step: d = A B.
+__device__ __forceinline__ void mma1688_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// The hi and lo fragments of two steps.
+struct FragA {
+    uint32_t h[2][4], l[2][4];
+};
+struct FragB {
+    uint32_t h[2][2], l[2][2];
+};
+// c[n] += A B[n] of two steps, the small terms first: the tensor core cuts its sums
+// off where fp32 rounds, so it sums sixteen products from zero and the long sum is an
+// fp32 addition.  Term by term over the N blocks: a block's six products wait for
+// one another, the blocks' do not.
+template <int N>
+__device__ __forceinline__ void mma_exact(float (*c)[4], const FragA& a, const FragB (&b)[N]) {
+    float d[N][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c[e] += d[e];
+    for (int n = 0; n < N; ++n) mma1688_first(d[n], a.l[0], b[n].h[0][0], b[n].h[0][1]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) mma1688(d[n], a.h[0], b[n].l[0][0], b[n].l[0][1]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) mma1688(d[n], a.l[1], b[n].h[1][0], b[n].h[1][1]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) mma1688(d[n], a.h[1], b[n].l[1][0], b[n].l[1][1]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) mma1688(d[n], a.h[0], b[n].h[0][0], b[n].h[0][1]);
+#pragma unroll
+    for (int n = 0; n < N; ++n) mma1688(d[n], a.h[1], b[n].h[1][0], b[n].h[1][1]);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[n][e] += d[n][e];
 }
 // 8x4 blocks of 32-bit words: lane's word is (lane / 4, lane % 4) of each block,
 // lane l gives the address of row l % 8 of block l / 8.
@@ -97,16 +127,18 @@ template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <int D, int FM, bool PREFIX>
-__global__ void __launch_bounds__(FT, (FM == 32 || D == 64) ? 2 : 1) paged_f32_kernel(const __grid_constant__ F32Args a) {
+__global__ void __launch_bounds__(FT, (FM == 32 || (FM == 64 && D == 64)) ? 2 : 1) paged_f32_kernel(const __grid_constant__ F32Args a) {
     using L = FLay<D, FM>;
+    constexpr int MR = L::MR;
     constexpr int NT = FN / L::WN / 8;                   // 8-key blocks of S per warp
     constexpr int CT = D / L::WN / 8;                    // 8-column blocks of O per warp
+    constexpr int NG = NT < 4 ? NT : 4, CG = CT < 4 ? CT : 4;    // blocks whose products interleave
     extern __shared__ __align__(16) float smf[];
     __shared__ SeqUnit s_seq;
     __shared__ int s_scan[FT / 32];
     float *sQ = smf + L::Q, *sK = smf + L::K, *sV = smf + L::V, *sP = smf + L::P, *sX = smf + L::X;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int wm = warp % L::WM, wn = warp / L::WM;      // the warp's 16 rows; its keys and columns
+    const int wm = warp % L::WM, wn = warp / L::WM;      // the warp's 16 MR rows; its keys and columns
     const int fr = lane >> 2, fc = lane & 3;             // row and word of a fragment
     if (PREFIX) pdl_trigger();
 
@@ -143,10 +175,17 @@ __global__ void __launch_bounds__(FT, (FM == 32 || D == 64) ? 2 : 1) paged_f32_k
     // ---- copies: four threads per key row
     const int cr = tid >> 2, cq = tid & 3;
     const uint32_t kdst = smem_u32(sK + cr * L::RS + cq * 4), vdst = smem_u32(sV + cr * L::RS + cq * 4);
-    auto place = [&](int j) -> long long {               // this thread's row of tile j in the pools, -1: zeros
+    // this thread's row of tile j: its page, looked up a tile before it is needed;
+    // its place in the pools, -1: zeros
+    auto seen = [&](int j, int row) { return j < n_kv && t.sees(row); };
+    auto look = [&](int j) {
         const int row = t.row0(j0 + j, FN) + cr;
-        if (j >= n_kv || !t.sees(row)) return -1;
-        const int page = checked_page(a.c, row_table[row >> a.c.page_log2]);
+        return seen(j, row) ? row_table[row >> a.c.page_log2] : 0;
+    };
+    auto place = [&](int j, int entry) -> long long {
+        const int row = t.row0(j0 + j, FN) + cr;
+        if (!seen(j, row)) return -1;
+        const int page = checked_page(a.c, entry);
         if (page < 0) return -1;
         return (long long)page * a.c.page_stride +
                (((long long)kvh << a.c.page_log2) + (row & ((1 << a.c.page_log2) - 1))) * D + cq * 4;
@@ -157,7 +196,9 @@ __global__ void __launch_bounds__(FT, (FM == 32 || D == 64) ? 2 : 1) paged_f32_k
         for (int c = 0; c < D / 16; ++c) cp16(dst + c * 64, at < 0 ? src : src + c * 16, at >= 0);
         cp_commit();
     };
-    long long at = place(0);
+    int entry = look(0);
+    const long long at = place(0, entry);
+    entry = look(1);
     if (n_kv > 0) {
         copy(kdst, a.c.k, at);
         copy(vdst, a.c.v, at);
@@ -181,119 +222,150 @@ __global__ void __launch_bounds__(FT, (FM == 32 || D == 64) ? 2 : 1) paged_f32_k
             make_float4(qv[u].x * a.qscale, qv[u].y * a.qscale, qv[u].z * a.qscale, qv[u].w * a.qscale);
     }
 
-    // what this lane's rows (fr and fr + 8 of the warp's) see
-    int lo[2], first[2];
-    unsigned span[2];
+    // what this lane's rows (fr and fr + 8 of each block) see
+    const int wr = wm * MR * 16 + fr;
+    int lo[2 * MR], first[2 * MR];
+    unsigned span[2 * MR];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int limit = PREFIX ? len - 1 : p0 + (wm * 16 + fr + 8 * i) / a.G;
+    for (int i = 0; i < 2 * MR; ++i) {
+        const int limit = PREFIX ? len - 1 : p0 + (wr + 8 * i) / a.G;
         lo[i] = PREFIX ? 0 : window_lo(limit, a.window);
         span[i] = limit < 0 ? 0u : (unsigned)(limit - lo[i] + 1);
         first[i] = PREFIX ? 0 : min(a.sinks, limit + 1);
     }
     const int all_lo = PREFIX ? 0 : window_lo(p0 + ntok - 1, a.window);
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[CT][4];
+    float m[2 * MR], l[2 * MR], o[MR][CT][4];
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
+    for (int i = 0; i < 2 * MR; ++i) m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[c][e] = 0.f;
+    for (int r = 0; r < MR; ++r)
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[r][c][e] = 0.f;
     // ldmatrix addresses: A (16 rows x 8 words): blocks by rows, then words; B (two
     // 8-key blocks x 8 words): blocks by words, then keys
-    const int ar = wm * 16 + (lane & 15), aw = (lane >> 4) * 4;
+    const int ar = wm * MR * 16 + (lane & 15), aw = (lane >> 4) * 4;
     const uint32_t qa = smem_u32(sQ + ar * L::RS + aw), pa = smem_u32(sP + ar * L::PS + aw);
     const uint32_t kb = smem_u32(sK + (wn * NT * 8 + (lane >> 4) * 8 + (lane & 7)) * L::RS + ((lane >> 3) & 1) * 4);
     // V: the eight keys of a step enter in the order that P's accumulator has them
     const uint32_t vb = smem_u32(sV + 2 * fc * L::RS + wn * CT * 8 + fr);
+    auto load_a = [&](FragA (&x)[MR], uint32_t at_, int stride) {
+#pragma unroll
+        for (int r = 0; r < MR; ++r)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t w[4];
+                ldsm4w(w, at_ + (r * 16 * stride + 8 * u) * 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) split_tf32(w[e], x[r].h[u][e], x[r].l[u][e]);
+            }
+    };
 
     for (int j = 0; j < n_kv; ++j) {
-        const long long next = place(j + 1);
+        const long long next = place(j + 1, entry);
+        entry = look(j + 2);
         cp_wait<1>();                                    // K of this tile (V is the group after it)
         __syncthreads();
-        float s[NT][4];
+        float s[MR][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int r = 0; r < MR; ++r)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-#pragma unroll 4
-        for (int k = 0; k < D; k += 8) {
-            uint32_t x[4], ah[4], al[4];
-            ldsm4w(x, qa + k * 4);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split_tf32(x[e], ah[e], al[e]);
+                for (int e = 0; e < 4; ++e) s[r][n][e] = 0.f;
+#pragma unroll 2
+        for (int k = 0; k < D; k += 16) {
+            FragA x[MR];
+            load_a(x, qa + k * 4, L::RS);
 #pragma unroll
-            for (int n = 0; n < NT; n += 2) {
-                uint32_t y[4], bh[4], bl[4];
-                ldsm4w(y, kb + (n * 8 * L::RS + k) * 4);
+            for (int n = 0; n < NT; n += NG) {
+                FragB y[NG];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) split_tf32(y[e], bh[e], bl[e]);
+                for (int i = 0; i < NG; i += 2)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    mma_exact(s[n + h], ah, al, bh[2 * h], bh[2 * h + 1], bl[2 * h], bl[2 * h + 1]);
-                }
+                    for (int u = 0; u < 2; ++u) {
+                        uint32_t w[4];
+                        ldsm4w(w, kb + ((n + i) * 8 * L::RS + k + 8 * u) * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            split_tf32(w[e], y[i + (e >> 1)].h[u][e & 1], y[i + (e >> 1)].l[u][e & 1]);
+                    }
+#pragma unroll
+                for (int r = 0; r < MR; ++r) mma_exact(s[r] + n, x[r], y);
             }
         }
         // accumulator: rows fr, fr + 8; keys 2 fc, 2 fc + 1 of each block
         const int k0 = t.row0(j0 + j, FN);
         if (k0 + FN - 1 > p0 || !(k0 >= all_lo || k0 + FN <= a.sinks)) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int r = 0; r < MR; ++r)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int key = k0 + (wn * NT + n) * 8 + 2 * fc + (e & 1), i = e >> 1;
-                    if ((unsigned)(key - lo[i]) >= span[i] && key >= first[i]) s[n][e] = -INFINITY;
-                }
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = k0 + (wn * NT + n) * 8 + 2 * fc + (e & 1), i = 2 * r + (e >> 1);
+                        if ((unsigned)(key - lo[i]) >= span[i] && key >= first[i]) s[r][n][e] = -INFINITY;
+                    }
         }
-        float mx[2];
+        float mx[2 * MR];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            mx[i] = fmaxf(s[0][2 * i], s[0][2 * i + 1]);
+        for (int i = 0; i < 2 * MR; ++i) {
+            const int r = i >> 1, e = 2 * (i & 1);
+            mx[i] = fmaxf(s[r][0][e], s[r][0][e + 1]);
 #pragma unroll
-            for (int n = 1; n < NT; ++n) mx[i] = fmaxf(mx[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]));
+            for (int n = 1; n < NT; ++n) mx[i] = fmaxf(mx[i], fmaxf(s[r][n][e], s[r][n][e + 1]));
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
             mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-            if (fc == 0) sX[wn * FM + wm * 16 + fr + 8 * i] = mx[i];
+            if (fc == 0) sX[wn * FM + wr + 8 * i] = mx[i];
         }
         __syncthreads();                                 // the other warps' maxima; everyone is done with K
         if (j + 1 < n_kv) copy(kdst, a.c.k, next);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2 * MR; ++i) {
+            const int r = i >> 1, e = 2 * (i & 1);
 #pragma unroll
-            for (int w = 0; w < L::WN; ++w) mx[i] = fmaxf(mx[i], sX[w * FM + wm * 16 + fr + 8 * i]);
+            for (int w = 0; w < L::WN; ++w) mx[i] = fmaxf(mx[i], sX[w * FM + wr + 8 * i]);
             const float M = fmaxf(m[i], mx[i]), z = M == -INFINITY ? 0.f : M;
             const float corr = ex2(m[i] - z);            // m = -inf: 0
             m[i] = M;
             float ps = 0.f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float p0_ = ex2(s[n][2 * i] - z), p1_ = ex2(s[n][2 * i + 1] - z);
+                const float p0_ = ex2(s[r][n][e] - z), p1_ = ex2(s[r][n][e + 1] - z);
                 ps += p0_ + p1_;
                 // key 2 fc goes to word fc of the step, key 2 fc + 1 to word fc + 4
-                float* dst = sP + (wm * 16 + fr + 8 * i) * L::PS + (wn * NT + n) * 8 + fc;
+                float* dst = sP + (wr + 8 * i) * L::PS + (wn * NT + n) * 8 + fc;
                 dst[0] = p0_;
                 dst[4] = p1_;
             }
             l[i] = l[i] * corr + ps;                     // this lane's keys; added up at the end
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-                o[c][2 * i] *= corr;
-                o[c][2 * i + 1] *= corr;
+                o[r][c][e] *= corr;
+                o[r][c][e + 1] *= corr;
             }
         }
         if (j + 1 < n_kv) cp_wait<1>();                  // V of this tile (K of the next came after it)
         else cp_wait<0>();
         __syncthreads();                                 // P and V are there
-#pragma unroll 4
-        for (int k = 0; k < FN; k += 8) {
-            uint32_t x[4], ah[4], al[4];
-            ldsm4w(x, pa + k * 4);
+#pragma unroll 2
+        for (int k = 0; k < FN; k += 16) {
+            FragA x[MR];
+            load_a(x, pa + k * 4, L::PS);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split_tf32(x[e], ah[e], al[e]);
+            for (int c = 0; c < CT; c += CG) {
+                FragB y[CG];
 #pragma unroll
-            for (int c = 0; c < CT; ++c) {
-                uint32_t bh[2], bl[2];
+                for (int i = 0; i < CG; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) split_tf32(lds32(vb + ((k + e) * L::RS + c * 8) * 4), bh[e], bl[e]);
-                mma_exact(o[c], ah, al, bh[0], bh[1], bl[0], bl[1]);
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            split_tf32(lds32(vb + ((k + 8 * u + e) * L::RS + (c + i) * 8) * 4), y[i].h[u][e],
+                                       y[i].l[u][e]);
+#pragma unroll
+                for (int r = 0; r < MR; ++r) mma_exact(o[r] + c, x[r], y);
             }
         }
         __syncthreads();                                 // V and P are free
@@ -302,15 +374,15 @@ __global__ void __launch_bounds__(FT, (FM == 32 || D == 64) ? 2 : 1) paged_f32_k
 
     // a row's sum: over its four lanes, then over the row group's warps
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2 * MR; ++i) {
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
         l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        if (fc == 0) sX[wn * FM + wm * 16 + fr + 8 * i] = l[i];
+        if (fc == 0) sX[wn * FM + wr + 8 * i] = l[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = wm * 16 + fr + 8 * i, tk = r / a.G, g = r - tk * a.G;
+    for (int i = 0; i < 2 * MR; ++i) {
+        const int r = wr + 8 * i, tk = r / a.G, g = r - tk * a.G;
         if (tk >= ntok) continue;
         float sum = 0.f;
 #pragma unroll
@@ -328,7 +400,8 @@ __global__ void __launch_bounds__(FT, (FM == 32 || D == 64) ? 2 : 1) paged_f32_k
         }
 #pragma unroll
         for (int c = 0; c < CT; ++c)
-            *reinterpret_cast<float2*>(dst + (wn * CT + c) * 8 + 2 * fc) = make_float2(o[c][2 * i] * f, o[c][2 * i + 1] * f);
+            *reinterpret_cast<float2*>(dst + (wn * CT + c) * 8 + 2 * fc) = 
+                make_float2(o[i >> 1][c][2 * (i & 1)] * f, o[i >> 1][c][2 * (i & 1) + 1] * f);
     }
 }
 
@@ -345,7 +418,9 @@ template <bool PREFIX>
 static int f32_launch(int d, int fm, cudaStream_t st, long long grid, const F32Args& a) {
     if (d == 64)
         return fm == 32 ? f32_launch_k<64, 32, PREFIX>(st, grid, a) : f32_launch_k<64, 64, PREFIX>(st, grid, a);
-    return fm == 32 ? f32_launch_k<128, 32, PREFIX>(st, grid, a) : f32_launch_k<128, 64, PREFIX>(st, grid, a);
+    return fm == 32   ? f32_launch_k<128, 32, PREFIX>(st, grid, a)
+           : fm == 64 ? f32_launch_k<128, 64, PREFIX>(st, grid, a)
+                      : f32_launch_k<128, 128, PREFIX>(st, grid, a);
 }
 
 int f32_prefill_launch(sa_ctx* ctx, const sa_paged_kv* kv, const float* q, long long q_tok, int n_tok, int hq,
@@ -360,18 +435,31 @@ int f32_prefill_launch(sa_ctx* ctx, const sa_paged_kv* kv, const float* q, long 
     // 64 rows read K and V half as often as 32; 32 where 64 would leave SMs idle
     const int seqs = std::min(kv->n_seqs, n_tok);
     auto units = [&](int fm) { return ((long long)n_tok / (fm / a.G) + seqs) * kv->hkv; };
-    const int fm = units(64) < 2 * ctx->num_sms ? 32 : 64;
+    int fm = units(64) < 2 * ctx->num_sms ? 32 : 64;
+    // 128 for d = 128 where the average sequence has 16 units of them (the last is
+    // partly empty) and they go round the SMs: 4096 tokens, 16/8 heads: 1260 us (64
+    // rows: 1520), 2048: 474 (598); not yet for 4 x 512 (eight units): 175 (147), nor
+    // for 8 x 130, 64/8 heads: 202 (182).  At d = 64 the halved splits do not pay for
+    // the halved occupancy: 701 (687)
+    if (kv->d == 128 && n_tok / seqs >= 16 * (128 / a.G) && 2 * units(128) >= 3 * ctx->num_sms) fm = 128;
     a.tpt = fm / a.G;
     return f32_launch<false>(kv->d, fm, ctx->stream, units(fm), a);
 }
 
-// Rows of a CTA behind a shared prefix: 32 where they hold all rows of a KV head.
-static int f32_prefix_rows(const sa_paged_kv* kv, int G) { return kv->n_seqs <= 32 / G ? 32 : 64; }
+// Rows of a CTA behind a shared prefix: 32 where they hold all rows of a KV head; 128
+// for d = 128 where that leaves no more rows empty than 64: 4000 rows, 200 query rows
+// per head: 98 us (64 rows: 125), 128: 64.6 (66.7); 144 would take two CTAs for three:
+// 95.6 (92.7).
+static int f32_prefix_rows(const sa_paged_kv* kv, int G) {
+    if (kv->n_seqs <= 32 / G) return 32;
+    auto units = [&](int fm) { return (kv->n_seqs + fm / G - 1) / (fm / G); };
+    return kv->d == 128 && 2 * units(128) <= units(64) + units(64) / 8 ? 128 : 64;
+}
 
 int f32_prefix_splits(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, int prefix_len) {
     const int G = hq / kv->hkv, fm = f32_prefix_rows(kv, G), tpt = fm / G, units = (kv->n_seqs + tpt - 1) / tpt;
     const int tiles = (int)(((long long)prefix_len + FN - 1) / FN);
-    const int slots = ctx->num_sms * ((kv->d == 64 || fm == 32) ? 2 : 1);
+    const int slots = ctx->num_sms * ((fm == 32 || (fm == 64 && kv->d == 64)) ? 2 : 1);
     return std::max(1, std::min(tiles, slots / std::max(1, units * kv->hkv)));
 }
 

@@ -314,6 +314,16 @@ def test_prefill_scores_of_all_sizes(dtype):
     assert (off <= (tolerance(dtype, ref, _v_max(pool)) if dtype == "bf16" else 0) + 1.5e-3 * _v_max(pool)).all()
 
 
+@pytest.mark.parametrize("hq,hkv,new,past", [(28, 14, [1100, 1001], [0, 70]), (32, 4, [700, 613, 500], [64, 0, 33]),
+                                             (24, 8, [900], [10]), (128, 8, [290, 0, 260], [100, 7, 0])])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 5)])
+def test_prefill_f32_long_chunks(hq, hkv, new, past, window, sinks):
+    """Chunks long enough for the widest row tile of fp32."""
+    pool = Pool([a + b for a, b in zip(past, new)], hkv, 128, 16, "f32", seed=hq)
+    out, ref = _prefill(pool, new, hq, window, sinks, tail=2)
+    _close(out, ref, "f32", _v_max(pool))
+
+
 def test_prefill_more_sequences_than_threads():
     new = [(5 * i) % 4 for i in range(900)]
     pool = Pool([n + i % 3 for i, n in enumerate(new)], 1, 64, 16, "bf16", seed=13)
@@ -379,6 +389,14 @@ def test_prefix(dtype, d, page, hq, hkv, n):
     lens = [(37 * i) % 90 for i in range(n)]               # 0 among them
     out, ref, v_max = _prefix(lens, 333, hq, hkv, d, page, dtype, seed=n)
     _close(out, ref, dtype, v_max)
+
+
+@pytest.mark.parametrize("hq,hkv,n", [(4, 2, 60), (3, 1, 80), (16, 1, 7), (1, 1, 500)])
+def test_prefix_f32_many_rows(hq, hkv, n):
+    """Rows that fill the widest row tile of fp32."""
+    for prefix in (1, 700):
+        out, ref, v_max = _prefix([(37 * i) % 90 for i in range(n)], prefix, hq, hkv, 128, 16, "f32", seed=n)
+        _close(out, ref, "f32", v_max)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
