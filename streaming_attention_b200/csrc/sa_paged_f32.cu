@@ -2,14 +2,7 @@
 // the prefill and the shared prefix's part of a decode, as sa_paged_tc.cu does
 // them for bf16.
 //
-// fp32 results from the tensor cores: an operand x is the sum of two tf32 numbers,
-// hi = x rounded to 11 significant bits and lo = x - hi (exact), and
-//   x y = hi hi' + hi lo' + lo hi'  (+ lo lo', at most 2^-22 of x y, left out),
-// each product exact in the fp32 accumulator; the tensor core drops lo's bits past
-// its eleventh, another 2^-22.  So three mma.m16n8k8 give what an fp32 FMA loop
-// gives to within its own rounding, at 512 / 3 FMA a clock and SM (measured)
-// where FMAs have 128 and spend half of their slots on feeding them.  (bf16
-// pairs would run twice as fast, at 2^-17.)
+// fp32 results from the tensor cores, three tf32 products each (sa_tf32.cuh).
 //
 // A CTA of eight warps holds FM query rows (FM / G tokens times the G heads of a
 // KV head) and walks over tiles of 64 keys: S = Q K^T with 16 rows per warp (32 at
@@ -31,6 +24,7 @@
 
 #include "sa_paged.cuh"
 #include "sa_paged_f32.h"
+#include "sa_tf32.cuh"
 
 namespace sa {
 namespace pg {
@@ -62,47 +56,11 @@ struct FLay {
     static constexpr int SMEM = (X + WN * FM) * 4;
 };
 
-__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t& hi, uint32_t& lo) {
-    hi = (x + 0x1000u) & 0xffffe000u;
-    lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
-}
-__device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// The product's first step: d = A B.
-__device__ __forceinline__ void mma1688_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-// The hi and lo fragments of two steps.
-struct FragA {
-    uint32_t h[2][4], l[2][4];
-};
-struct FragB {
-    uint32_t h[2][2], l[2][2];
-};
-// c[n] += A B[n] of two steps, the small terms first: the tensor core cuts its sums
-// off where fp32 rounds, so it sums sixteen products from zero and the long sum is an
-// fp32 addition.  Term by term over the N blocks: a block's six products wait for
-// one another, the blocks' do not.
+// c[n] += A B[n] of sixteen products.
 template <int N>
-__device__ __forceinline__ void mma_exact(float (*c)[4], const FragA& a, const FragB (&b)[N]) {
+__device__ __forceinline__ void add_product(float (*c)[4], const FragA<2>& a, const FragB<2> (&b)[N]) {
     float d[N][4];
-#pragma unroll
-    for (int n = 0; n < N; ++n) mma1688_first(d[n], a.l[0], b[n].h[0][0], b[n].h[0][1]);
-#pragma unroll
-    for (int n = 0; n < N; ++n) mma1688(d[n], a.h[0], b[n].l[0][0], b[n].l[0][1]);
-#pragma unroll
-    for (int n = 0; n < N; ++n) mma1688(d[n], a.l[1], b[n].h[1][0], b[n].h[1][1]);
-#pragma unroll
-    for (int n = 0; n < N; ++n) mma1688(d[n], a.h[1], b[n].l[1][0], b[n].l[1][1]);
-#pragma unroll
-    for (int n = 0; n < N; ++n) mma1688(d[n], a.h[0], b[n].h[0][0], b[n].h[0][1]);
-#pragma unroll
-    for (int n = 0; n < N; ++n) mma1688(d[n], a.h[1], b[n].h[1][0], b[n].h[1][1]);
+    mma_exact(d, [&](int) -> const FragA<2>& { return a; }, b);
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -250,7 +208,7 @@ __global__ void __launch_bounds__(FT, (FM == 32 || (FM == 64 && D == 64)) ? 2 : 
     const uint32_t kb = smem_u32(sK + (wn * NT * 8 + (lane >> 4) * 8 + (lane & 7)) * L::RS + ((lane >> 3) & 1) * 4);
     // V: the eight keys of a step enter in the order that P's accumulator has them
     const uint32_t vb = smem_u32(sV + 2 * fc * L::RS + wn * CT * 8 + fr);
-    auto load_a = [&](FragA (&x)[MR], uint32_t at_, int stride) {
+    auto load_a = [&](FragA<2> (&x)[MR], uint32_t at_, int stride) {
 #pragma unroll
         for (int r = 0; r < MR; ++r)
 #pragma unroll
@@ -276,11 +234,11 @@ __global__ void __launch_bounds__(FT, (FM == 32 || (FM == 64 && D == 64)) ? 2 : 
                 for (int e = 0; e < 4; ++e) s[r][n][e] = 0.f;
 #pragma unroll 2
         for (int k = 0; k < D; k += 16) {
-            FragA x[MR];
+            FragA<2> x[MR];
             load_a(x, qa + k * 4, L::RS);
 #pragma unroll
             for (int n = 0; n < NT; n += NG) {
-                FragB y[NG];
+                FragB<2> y[NG];
 #pragma unroll
                 for (int i = 0; i < NG; i += 2)
 #pragma unroll
@@ -292,7 +250,7 @@ __global__ void __launch_bounds__(FT, (FM == 32 || (FM == 64 && D == 64)) ? 2 : 
                             split_tf32(w[e], y[i + (e >> 1)].h[u][e & 1], y[i + (e >> 1)].l[u][e & 1]);
                     }
 #pragma unroll
-                for (int r = 0; r < MR; ++r) mma_exact(s[r] + n, x[r], y);
+                for (int r = 0; r < MR; ++r) add_product(s[r] + n, x[r], y);
             }
         }
         // accumulator: rows fr, fr + 8; keys 2 fc, 2 fc + 1 of each block
@@ -351,11 +309,11 @@ __global__ void __launch_bounds__(FT, (FM == 32 || (FM == 64 && D == 64)) ? 2 : 
         __syncthreads();                                 // P and V are there
 #pragma unroll 2
         for (int k = 0; k < FN; k += 16) {
-            FragA x[MR];
+            FragA<2> x[MR];
             load_a(x, pa + k * 4, L::PS);
 #pragma unroll
             for (int c = 0; c < CT; c += CG) {
-                FragB y[CG];
+                FragB<2> y[CG];
 #pragma unroll
                 for (int i = 0; i < CG; ++i)
 #pragma unroll
@@ -365,7 +323,7 @@ __global__ void __launch_bounds__(FT, (FM == 32 || (FM == 64 && D == 64)) ? 2 : 
                             split_tf32(lds32(vb + ((k + 8 * u + e) * L::RS + (c + i) * 8) * 4), y[i].h[u][e],
                                        y[i].l[u][e]);
 #pragma unroll
-                for (int r = 0; r < MR; ++r) mma_exact(o[r] + c, x[r], y);
+                for (int r = 0; r < MR; ++r) add_product(o[r] + c, x[r], y);
             }
         }
         __syncthreads();                                 // V and P are free

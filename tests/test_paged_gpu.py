@@ -187,6 +187,17 @@ def test_decode_window(dtype, d, page, window, sinks):
     _close(out, ref, dtype, _v_max(pool), (window, sinks))
 
 
+@pytest.mark.parametrize("hq,hkv,d,page", [(5, 1, 64, 16), (16, 2, 128, 32), (14, 2, 256, 16), (16, 1, 64, 64), (22, 2, 128, 16)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (40, 3), (0, 0), (200, 70)])
+def test_decode_f32_many_heads(hq, hkv, d, page, window, sinks):
+    """More than four heads per KV head: masked rows inside a block of eight, freed pages, NaN behind the end."""
+    pool = Pool(LENS + [1000], hkv, d, page, "f32", seed=hq + sinks)
+    for b, n in enumerate(pool.lens):
+        pool.forget(b, lambda r, n=n: sees(n - 1, r, window, sinks))
+    out, ref = _decode(pool, hq, window, sinks, q_pad=1)
+    _close(out, ref, "f32", _v_max(pool), (window, sinks))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_decode_scores_of_all_sizes(dtype):
     """Logits with a spread of hundreds: the running maximum moves many times."""
