@@ -376,6 +376,11 @@ int sa_attn_decode_noalloc(void* stream, int dtype, const void* q, const void* k
  * accessed (its rows' contribution is undefined), and sa_ctx_synchronize then
  * returns SA_ERR_RANGE.
  *
+ * fp32 products run on the tensor cores in the prefill, behind a shared prefix
+ * and in decodes with more than four query heads per KV head: each operand as
+ * the sum of two tf32 numbers, which keeps fp32's precision for magnitudes from
+ * 2^-100 to 2^127 (smaller ones lose bits, larger ones may overflow).
+ *
  * Workspaces are the caller's (256-byte aligned device memory); calls that may
  * run at the same time, captured ones included, need workspaces of their own.
  * Their sizes depend on the shapes in kv, on hq and on the prefix's length, not
@@ -446,7 +451,7 @@ int sa_attn_paged_decode(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long
  * elements), tokens cu_q[b] .. cu_q[b+1] - 1 the last ones of sequence b
  * (token t of n at position kv_lens[b] - n + t), whose keys and values are in
  * the pages.  Causal, with the window above.  bf16 on the tensor cores
- * (softmax weights in bf16, sums in fp32), fp32 on CUDA cores.  d 64 or 128.
+ * (softmax weights in bf16, sums in fp32), fp32 there too (above).  d 64 or 128.
  * Rows behind the last sequence are left as they were.
  */
 int sa_attn_paged_prefill(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_tok_stride, int n_tokens,

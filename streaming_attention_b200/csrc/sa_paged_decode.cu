@@ -662,8 +662,8 @@ struct FGeo {
     static constexpr int CPL = D / 8, CH = CPL / 4;        // columns per lane, as CH float4
 };
 // CTAs per SM: two where their registers (q and O: 2 HG D / 8 a thread) fit.
-template <int D, int HG, int NG>
-constexpr int f32_ctas() { return (NG == 1 || (NG == 2 && HG * D <= 256)) ? 2 : 1; }
+template <int NG>
+constexpr int f32_ctas() { return NG == 1 ? 2 : 1; }
 template <int D, int HG, int NG>
 constexpr int f32_smem() {
     return STAGES * Geo<float, D>::STAGE_BYTES + NG * 4 * HG * (D + 2) * 4 + 128;
@@ -711,7 +711,7 @@ __device__ __forceinline__ void finish_f32(const DecodeArgs& a, Ring* r, const S
 }
 
 template <int D, int HG, int NG>
-__global__ void __launch_bounds__((NG * 4 + 1) * 32, f32_ctas<D, HG, NG>())
+__global__ void __launch_bounds__((NG * 4 + 1) * 32, f32_ctas<NG>())
 decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
     using Z = Geo<float, D>;
     using F = FGeo<D>;
@@ -1161,7 +1161,7 @@ struct F32Pick {
 };
 template <int D, int HG, int NG>
 static F32Pick f32_pick() {
-    return {decode_f32_kernel<D, HG, NG>, (NG * 4 + 1) * 32, f32_smem<D, HG, NG>(), f32_ctas<D, HG, NG>()};
+    return {decode_f32_kernel<D, HG, NG>, (NG * 4 + 1) * 32, f32_smem<D, HG, NG>(), f32_ctas<NG>()};
 }
 template <int D, int MH>
 static F32Pick f32_heads_pick() {

@@ -44,7 +44,6 @@
 
 #include "sa_fa.cuh"
 #include "sa_paged.cuh"
-#include "sa_paged_decode.h"
 #include "sa_paged_tc.h"
 
 namespace sa {

@@ -458,6 +458,25 @@ def test_a_bad_page_fails_no_later_call():
         assert torch.isfinite(out).all() and torch.isfinite(good).all()
 
 
+@pytest.mark.parametrize("power", [-70, 100])
+def test_f32_magnitudes(power):
+    """Values of 2^-70 and 2^100 through the fp32 products keep their precision: the exact scaled result."""
+    sa = _sa()
+    pool = Pool([300, 40, 130, 77], 1, 128, 16, "f32", seed=21)
+    pool.vp.mul_(2.0 ** power)
+    new = [100, 40, 0, 3]
+    cu = torch.tensor([0] + new).cumsum(0)
+    scale = 1.0 / math.sqrt(128)
+    q = pool.q(sum(new), 8)
+    out = sa.attn_paged_prefill(q.cuda(), pool.kp, pool.vp, pool.table, pool.kv_lens, cu.int().cuda(), scale)
+    ref = torch.cat([attend(q[cu[b]:cu[b + 1]], pool.k[b], pool.v[b], list(range(m - new[b], m)), scale)
+                     for b, m in enumerate(pool.lens)])
+    _close(out.double() * 2.0 ** -power, ref, "f32", _v_max(pool))
+    out = sa.attn_paged_decode(q[:4].cuda(), pool.kp, pool.vp, pool.table, pool.kv_lens, scale)
+    ref = torch.cat([attend(q[b:b + 1], pool.k[b], pool.v[b], [m - 1], scale) for b, m in enumerate(pool.lens)])
+    _close(out.double() * 2.0 ** -power, ref, "f32", _v_max(pool))
+
+
 # ---------------------------------------------------------------- together
 
 def _rope_ref(cos, sin, rot, x, pos, dt):
