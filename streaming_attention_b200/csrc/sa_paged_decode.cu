@@ -37,10 +37,11 @@
 // up to 8191 rows, 16/8 heads (0.68 GB): 108-114 us.  One sequence of 32768 rows
 // (134 MB): 34 us -- some 10 us go to the plan, the first table entry and copy, and
 // the join, which follow one another.  fp32, 16 sequences of up to 4000 rows, 8 KV
-// heads of 128 (0.41 GB): 69 / 72 / 85 us for 1 / 2 / 4 heads each on FMAs, 97 for
-// eight and 122 for sixteen on tensor cores (127 and 411 on FMAs, whose q and O did
-// not fit the registers); 64/8 heads of 64: 87 (133), of 256: 167 (286).  There the
-// chains of dependent products of 4 to 8 warps per SM bind.
+// heads of 128 (0.41 GB): 69 / 72 / 85 us for 1 / 2 / 4 heads each on FMAs, 91 for
+// eight and 119 for sixteen on tensor cores (127 and 411 on FMAs, whose q and O did
+// not fit the registers); 64/8 heads of 64: 87 (133), of 256: 157 (286).  There the
+// chains of dependent products of 4 to 8 warps per SM bind (tensor pipe 0.4 busy,
+// half of the issue slots).
 #include <cuda_bf16.h>
 #include <algorithm>
 #include <cmath>
@@ -901,17 +902,11 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
 // MH blocks of eight heads on the tensor cores, three tf32 products each: S = q K^T
 // with the heads as the matrix's M (so P is an operand as it stands) and eight rows as
 // its N; O += P V with eight columns as N and the rows as K.
-// x's bits, for arithmetic that is not to be moved out of a loop (and kept in registers).
-__device__ __forceinline__ uint32_t keep_here(float x) {
-    uint32_t y = __float_as_uint(x);
-    asm volatile("" : "+r"(y));
-    return y;
-}
 template <int D, int MH>
 struct TGeo {
     using Z = Geo<float, D>;
     static constexpr int NW = Z::TK >= 32 ? 4 : 2, RW = Z::TK / NW, NB = RW / 8;   // warps, their rows, in eights
-    static constexpr int CTAS = MH * D <= 128 || (MH == 1 && NW == 2) ? 2 : 1;     // q and O: MH D / 2 a thread
+    static constexpr int CTAS = MH * D <= 128 || (MH == 1 && NW == 2) ? 2 : 1;     // O: MH D / 4 a thread
     static constexpr int SMEM = STAGES * Z::STAGE_BYTES + NW * 8 * MH * (D + 2) * 4 + 128;
 };
 
@@ -958,25 +953,22 @@ decode_f32_heads_kernel(const __grid_constant__ DecodeArgs a) {
     // The sum's order is free, so those words are four neighbouring columns of a
     // sixteen for two steps, one 16-byte load of q and of K.
     const int fr = lane >> 2, fc = lane & 3;
-    float q[MH][D / 4];
-    auto load_q = [&](int b, int h) {
+    // Both halves of q, as the lanes take them, lie where the pair's states go in the
+    // end (they are the same for all warps, and split once a pair).
+    constexpr int QN = MH * D / 16 / NW;
+    uint4* qs = reinterpret_cast<uint4*>(red);               // [MH][D / 16][hi, lo][lane]
+    float4 nq[QN];                                           // this warp's part of the next pair's
+    auto fetch_q = [&](int b, int h) {
 #pragma unroll
-        for (int n = 0; n < MH; ++n) {
-            const int g = n * 8 + fr;
-            const float f = g < a.G ? a.qscale : 0.f;
-            const float* qh = static_cast<const float*>(a.q) + (long long)b * a.q_stride +
-                              (long long)(h * a.G + (g < a.G ? g : 0)) * D + fc * 4;
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-                const float4 x = *reinterpret_cast<const float4*>(qh + c * 16);
-                q[n][c * 4] = x.x * f;
-                q[n][c * 4 + 1] = x.y * f;
-                q[n][c * 4 + 2] = x.z * f;
-                q[n][c * 4 + 3] = x.w * f;
-            }
+        for (int u = 0; u < QN; ++u) {
+            const int i = warp * QN + u, n = i / (D / 16), c = i % (D / 16), g = n * 8 + fr;
+            nq[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (g < a.G)
+                nq[u] = *reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (long long)b * a.q_stride +
+                                                         (long long)(h * a.G + g) * D + c * 16 + fc * 4);
         }
     };
-    load_q(w.b, w.h);
+    fetch_q(w.b, w.h);
     int it = 0;
     bool ok = true;
     while (w.left > 0) {
@@ -984,6 +976,17 @@ decode_f32_heads_kernel(const __grid_constant__ DecodeArgs a) {
         const Tiles t = w.t;
         const int i1 = min(t.n, i0 + w.left);
         const long long seg_first = sh.first + (sh.count - w.left);
+#pragma unroll
+        for (int u = 0; u < QN; ++u) {
+            uint4 hi, lo;
+            split_tf32(__float_as_uint(nq[u].x * a.qscale), hi.x, lo.x);
+            split_tf32(__float_as_uint(nq[u].y * a.qscale), hi.y, lo.y);
+            split_tf32(__float_as_uint(nq[u].z * a.qscale), hi.z, lo.z);
+            split_tf32(__float_as_uint(nq[u].w * a.qscale), hi.w, lo.w);
+            qs[(warp * QN + u) * 64 + lane] = hi;
+            qs[(warp * QN + u) * 64 + 32 + lane] = lo;
+        }
+        bar_consumers<NW * 32>();
         // O: heads fr + 8 n, columns 8 c + 2 fc, + 1
         float o[D / 8][2 * MH], m[MH], l[MH];
 #pragma unroll
@@ -1034,15 +1037,17 @@ decode_f32_heads_kernel(const __grid_constant__ DecodeArgs a) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                                for (int n = 0; n < 2; ++n) {
-                                    uint32_t &hi = qf[u].h[k][2 * e + n], &lo = qf[u].l[k][2 * e + n];
-                                    if (n < MH) split_tf32(keep_here(q[n][(c + u) * 4 + 2 * k + e]), hi, lo);
-                                    else hi = lo = 0;
-                                }
+                        for (int n = 0; n < 2; ++n) {
+                            uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+                            if (n < MH) {
+                                hi = qs[(n * (D / 16) + c + u) * 64 + lane];
+                                lo = qs[(n * (D / 16) + c + u) * 64 + 32 + lane];
+                            }
+                            qf[u].h[0][n] = hi.x; qf[u].h[0][2 + n] = hi.y;
+                            qf[u].h[1][n] = hi.z; qf[u].h[1][2 + n] = hi.w;
+                            qf[u].l[0][n] = lo.x; qf[u].l[0][2 + n] = lo.y;
+                            qf[u].l[1][n] = lo.z; qf[u].l[1][2 + n] = lo.w;
+                        }
                     float d[4][4];
                     mma_exact(d, [&](int n) -> const FragA<2>& { return qf[n]; }, kf);
 #pragma unroll
@@ -1136,7 +1141,8 @@ decode_f32_heads_kernel(const __grid_constant__ DecodeArgs a) {
         }
         const bool whole = i0 == 0 && i1 == t.n;
         const Dest ds = segment_dest(a, sh, seg_first, whole, b, h);
-        if (w.left > 0) load_q(w.b, w.h);
+        if (w.left > 0) fetch_q(w.b, w.h);
+        bar_consumers<NW * 32>();                            // everyone is done with q
 #pragma unroll
         for (int n = 0; n < MH; ++n) {
             l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
@@ -1171,7 +1177,7 @@ static F32Pick f32_heads_pick() {
 template <int D>
 static F32Pick f32_pick_g(int G) {
     // the tensor cores take as long for one head as for eight: 16 sequences of up to 4000
-    // rows, 8 KV heads of 128: 94-97 us, FMAs 72 / 85 / 126 us at 2 / 4 / 8 heads each
+    // rows, 8 KV heads of 128: 90 us, FMAs 72 / 85 / 126 us at 2 / 4 / 8 heads each
     if (G > 8) return f32_heads_pick<D, (D <= 128 ? 2 : 1)>();       // d = 256 has at most 8
     if (G > 4) return f32_heads_pick<D, 1>();
     if (G == 1) return f32_pick<D, 1, 1>();

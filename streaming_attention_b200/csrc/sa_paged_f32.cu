@@ -13,7 +13,7 @@
 // the next S; the page of the tile after it is looked up meanwhile.  Rows that no
 // query of the CTA sees are not read but zero-filled.
 //
-// Bound: the tensor pipe (0.60 busy over 4096 causal tokens) with the splits and the
+// Bound: the tensor pipe (0.63 busy over 4096 causal tokens) with the splits and the
 // softmax between its products; small calls by the latency of few dependent tiles.
 // Measured: 16 sequences behind 4001 rows, 16/8 heads of 128: 22.9 us for the
 // prefix (42 on FMAs); three chunks of up to 300 tokens, 8/4 heads of 64, window

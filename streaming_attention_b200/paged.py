@@ -13,6 +13,9 @@ the pages' device, asynchronously.
   cu_q              [n_seqs + 1] int32: sequence b's tokens are rows
                     cu_q[b] .. cu_q[b + 1] - 1 of the token tensors
 
+A context, the default one of a GPU included, serves one thread at a time;
+threads that call at once pass one each as ``ctx``.
+
 Workspaces come from torch's allocator: calls on different streams and calls
 captured into different graphs do not share one.
 
