@@ -163,6 +163,7 @@ class Context:
 
     def __init__(self, device: int = 0):
         self.device = device
+        self.workspaces: dict = {}      # torch buffers that operators keep from call to call, by stream
         h = _vp()
         check(lib().sa_ctx_create(device, C.byref(h)))
         self.h = h
@@ -171,6 +172,7 @@ class Context:
         if getattr(self, "h", None):
             lib().sa_ctx_destroy(self.h)
             self.h = None
+            self.workspaces.clear()
 
     def __del__(self):
         try:

@@ -31,9 +31,12 @@ int decode_grid(const sa_ctx* ctx, const sa_paged_kv* kv, int hq);
 // with room for whole pairs' states.
 size_t decode_ws_layout(const sa_ctx* ctx, const sa_paged_kv* kv, int hq, bool prefix, void* base, DecodeWs* ws);
 // prefix (may be null): the rows of a shared prefix come before each sequence's
-// own.  Where it has parts, the stream's last kernel is the one that computes
-// them, which started after everything else that this launch reads was written:
-// the launch may start while it runs, and waits for it before it joins.
+// own.  Where it has parts, the kernel that computes them is before this launch on
+// the stream, and started after everything else that the launch reads was written:
+// the launch may start while it runs, and waits for it before it joins.  Kernels
+// that other threads enqueued may lie between the two: each ends after the one
+// before it, so the wait (for the last of them) covers the parts, and they have
+// workspaces of their own.
 int decode_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_stride, int hq, int window, int sinks,
                   float scale, void* out, long long o_stride, const PrefixParts* prefix, const DecodeWs& ws);
 

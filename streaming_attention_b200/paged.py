@@ -16,8 +16,8 @@ the pages' device, asynchronously.
 A context, the default one of a GPU included, serves one thread at a time;
 threads that call at once pass one each as ``ctx``.
 
-Workspaces come from torch's allocator: calls on different streams and calls
-captured into different graphs do not share one.
+Workspaces come from torch's allocator: calls with different contexts, calls on
+different streams and calls captured into different graphs do not share one.
 
 A decode step of a small batch takes the GPU some ten microseconds, so the
 wrappers are written to cost the host less than that: one look at each
@@ -34,7 +34,6 @@ from ._capi import SA_BF16, SA_F32, SA_PAGED_ZERO_BYTES, Context, check, default
 _torch = None
 _lib = None
 _sizes: dict = {}
-_kept: dict = {}
 # the members of sa_paged_kv in order, natively aligned
 _pack = struct.Struct("@PPiiiiiqPqiPi").pack
 
@@ -107,14 +106,14 @@ def _cache(k_pages, v_pages, block_table, kv_lens):
     return kv, dev, dt, code, hkv, d, page, n_seqs
 
 
-def _bind(ctx: Context | None, dev: int):
-    """The handle of the context, bound to torch's current stream of its GPU."""
+def _bind(ctx: Context | None, dev: int) -> Context:
+    """The context, bound to torch's current stream of its GPU."""
     if ctx is None:
         ctx = default_context(dev)
     elif ctx.device != dev:
         raise ValueError(f"the context is on GPU {ctx.device}, the pages on GPU {dev}")
     check(_lib.sa_ctx_set_stream(ctx.h, _torch._C._cuda_getCurrentRawStream(dev)))
-    return ctx.h
+    return ctx
 
 
 def _size(key, size_fn, *args) -> int:
@@ -128,16 +127,22 @@ def _size(key, size_fn, *args) -> int:
     return n
 
 
-def _workspace(dev: int, n: int):
-    """A decode's workspace, its head zero: kept from call to call of a stream; a captured call has its own."""
+def _workspace(ctx: Context, dev: int, n: int):
+    """A decode's workspace, its head zero; a captured call has its own.
+
+    Kept from call to call of one context on one stream: those follow one another.
+    Calls of threads that share a stream (torch's default one, unless they set
+    another) do not: they have a context each, and a call may be several launches,
+    which pass states through the workspace while another call's lie between them.
+    """
     if _torch._C._cuda_isCurrentStreamCapturing():
         ws = _torch.empty(n, dtype=_torch.uint8, device=dev)
         ws[:SA_PAGED_ZERO_BYTES].zero_()
         return ws
-    key = (dev, _torch._C._cuda_getCurrentRawStream(dev))
-    ws = _kept.get(key)
+    stream = _torch._C._cuda_getCurrentRawStream(dev)
+    ws = ctx.workspaces.get(stream)
     if ws is None or ws.numel() < n:
-        ws = _kept[key] = _torch.zeros(n, dtype=_torch.uint8, device=dev)
+        ws = ctx.workspaces[stream] = _torch.zeros(n, dtype=_torch.uint8, device=dev)
     return ws
 
 
@@ -148,7 +153,7 @@ def rope_table(theta: float, rotary_dim: int, n_pos: int, device="cuda", ctx: Co
     dev = device.index if device.index is not None else torch.cuda.current_device()
     cos = torch.empty(n_pos, rotary_dim // 2, dtype=torch.float32, device=torch.device("cuda", dev))
     sin = torch.empty_like(cos)
-    check(_lib.sa_rope_table(_bind(ctx, dev), n_pos, rotary_dim, theta, cos.data_ptr(), sin.data_ptr()))
+    check(_lib.sa_rope_table(_bind(ctx, dev).h, n_pos, rotary_dim, theta, cos.data_ptr(), sin.data_ptr()))
     return cos, sin
 
 
@@ -189,7 +194,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, kv_lens, cu_q=None, q=None
             if x.dtype is not _torch.float32 or x.shape != cos.shape or x.get_device() != dev or not x.is_contiguous():
                 raise ValueError(f"rope: want contiguous float32 {tuple(cos.shape)} on GPU {dev}")
         cosp, sinp = cos.data_ptr(), sin.data_ptr()
-    check(_lib.sa_paged_append(_bind(ctx, dev), kv, _code(k, "k"), qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, n, hq, cp,
+    check(_lib.sa_paged_append(_bind(ctx, dev).h, kv, _code(k, "k"), qp, qs, k.data_ptr(), ks, v.data_ptr(), vs, n, hq, cp,
                                pos0, cosp, sinp, n_pos, rot, 1 if interleaved else 0, qop, os))
     return q_out
 
@@ -210,10 +215,10 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, kv_lens, scale: float, w
         out, os = _torch.empty_like(q, memory_format=_torch.contiguous_format), hq * d
     else:
         os = _rows(out, "out", n_seqs, hq, d, dev, dt)
-    h = _bind(ctx, dev)
-    n = _size((dev, code, hkv, hq, d), _lib.sa_attn_paged_decode_workspace, h, kv, hq)
-    ws = _workspace(dev, n)
-    check(_lib.sa_attn_paged_decode(h, kv, q.data_ptr(), qs, hq, window, sinks, scale, out.data_ptr(), os, ws.data_ptr(), n))
+    ctx = _bind(ctx, dev)
+    n = _size((dev, code, hkv, hq, d), _lib.sa_attn_paged_decode_workspace, ctx.h, kv, hq)
+    ws = _workspace(ctx, dev, n)
+    check(_lib.sa_attn_paged_decode(ctx.h, kv, q.data_ptr(), qs, hq, window, sinks, scale, out.data_ptr(), os, ws.data_ptr(), n))
     return out
 
 
@@ -236,7 +241,7 @@ def attn_paged_prefill(q, k_pages, v_pages, block_table, kv_lens, cu_q, scale: f
         out, os = _torch.empty_like(q, memory_format=_torch.contiguous_format), hq * d
     else:
         os = _rows(out, "out", n, hq, d, dev, dt)
-    check(_lib.sa_attn_paged_prefill(_bind(ctx, dev), kv, q.data_ptr(), qs, n, hq, cp, window, sinks, scale,
+    check(_lib.sa_attn_paged_prefill(_bind(ctx, dev).h, kv, q.data_ptr(), qs, n, hq, cp, window, sinks, scale,
                                      out.data_ptr(), os))
     return out
 
@@ -260,9 +265,9 @@ def attn_paged_decode_prefix(q, k_pages, v_pages, prefix_table, prefix_len: int,
         out, os = _torch.empty_like(q, memory_format=_torch.contiguous_format), hq * d
     else:
         os = _rows(out, "out", n_seqs, hq, d, dev, dt)
-    h = _bind(ctx, dev)
-    n = _size((dev, code, hkv, hq, d, n_seqs, prefix_len), _lib.sa_attn_paged_decode_prefix_workspace, h, kv, hq, prefix_len)
-    ws = _workspace(dev, n)
-    check(_lib.sa_attn_paged_decode_prefix(h, kv, pp, prefix_len, q.data_ptr(), qs, hq, scale, out.data_ptr(), os,
+    ctx = _bind(ctx, dev)
+    n = _size((dev, code, hkv, hq, d, n_seqs, prefix_len), _lib.sa_attn_paged_decode_prefix_workspace, ctx.h, kv, hq, prefix_len)
+    ws = _workspace(ctx, dev, n)
+    check(_lib.sa_attn_paged_decode_prefix(ctx.h, kv, pp, prefix_len, q.data_ptr(), qs, hq, scale, out.data_ptr(), os,
                                            ws.data_ptr(), n))
     return out
