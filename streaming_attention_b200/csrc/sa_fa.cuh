@@ -32,6 +32,12 @@ __device__ __forceinline__ bool wait_ab(uint64_t* bar, uint32_t parity, volatile
     return true;
 }
 
+// The same for a whole (converged) warp: its lanes look at the barrier and the clock
+// one by one, and go on together or give up together.
+__device__ __forceinline__ bool wait_ab_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int* status) {
+    return __all_sync(0xffffffffu, wait_ab(bar, parity, abort, status));
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);

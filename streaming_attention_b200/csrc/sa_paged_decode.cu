@@ -246,11 +246,16 @@ struct Ring {
     int last;                // this CTA handed in a pair's last share
 };
 
+// A wait of a whole (converged) warp: its lanes look at the barrier and the clock
+// one by one, and go on together or give up together.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
+}
 // A consumer warp's wait for tile `it` of its share; the first that expires is
 // noted, and no further one is waited for.
 __device__ __forceinline__ bool consume_wait(Ring* r, int it, bool& ok, int* status) {
     if (!ok) return false;
-    if ((ok = mbar_wait(r->full + it % STAGES, (it / STAGES) & 1, status))) return true;
+    if ((ok = mbar_wait_warp(r->full + it % STAGES, (it / STAGES) & 1, status))) return true;
     atomicMin(&r->consumed, it);
     r->failed = 1;
     return false;
@@ -336,7 +341,7 @@ __device__ __forceinline__ void produce(const CUtensorMap* tk, const CUtensorMap
         w.next(a, TK);
         if (it + 1 < n) entry = lookup(w);
         const int s = it % STAGES;
-        if (it >= STAGES && !mbar_wait(r->empty + s, ((it / STAGES) & 1) ^ 1, a.c.status)) break;
+        if (it >= STAGES && !mbar_wait_warp(r->empty + s, ((it / STAGES) & 1) ^ 1, a.c.status)) break;
         const unsigned got = __ballot_sync(0xffffffffu, page_id >= 0);
         const uint32_t bytes = (uint32_t)(rows * D * Z::ELT);
         if (lane == 0) mbar_arrive_expect_tx(r->full + s, 2 * __popc(got) * bytes);

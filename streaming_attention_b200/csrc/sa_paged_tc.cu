@@ -55,6 +55,7 @@ using pf::col_o;
 using pf::col_p;
 using pf::col_s;
 using pf::wait_ab;
+using pf::wait_ab_warp;
 
 constexpr int TC_THREADS = 384;
 constexpr int TC_REG_CTRL = 72, TC_REG_SOFTMAX = 216;      // 128 * 72 + 256 * 216 = 384 * 168
@@ -253,8 +254,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                     if (pg_id < 0) pg_id = a.c.n_pages;
                 }
                 if (j + 1 < n_kv) next = entry(j + 1);
-                const bool ok = j < ST || wait_ab(&empty[s], ((j / ST) & 1) ^ 1, abort, status);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                if (j >= ST && !wait_ab_warp(&empty[s], ((j / ST) & 1) ^ 1, abort, status)) break;
                 if (lane == 0) mbar_arrive_expect_tx(&full[s], L::TILE);
                 __syncwarp();
                 if (lane < copies)
@@ -383,6 +383,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
             const float sl2 = a.sl2;
             const int j0 = s_unit.j0;
             float m = -INFINITY, l = 0.f;
+            // A lane whose wait expired goes on, without further waits, over whatever S and V
+            // hold: the warp stays together at every vote and TMEM access (and needs no vote
+            // of its own per wait: with one, 1.5% more time).  The row is given up at the end.
             bool ok = true;
             for (int c = 0; c < nx; ++c) {
                 // what needs no score is settled before the wait for them
@@ -392,7 +395,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                 // the first slot that uses a tile with rows behind the last one clears
                 // them in V: they enter P.V as zeros (the other's P.V is issued later)
                 const bool clear = k0 + BN > len && (ALT || x == 0 || j >= n0);
-                if (!(ok = wait_ab(&B->s_full[x], c & 1, abort, status))) break;
+                ok = ok && wait_ab(&B->s_full[x], c & 1, abort, status);
                 tc::fence_after_sync();
                 uint32_t u32[BN];
 #pragma unroll
@@ -428,7 +431,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                 }
                 if (clear) {
                     const int s = j % ST, r0 = max(0, len - k0), n = (BN - r0) * 8 * L::HALVES;
-                    if (!(ok = wait_ab(&B->v_full[s], (j / ST) & 1, abort, status))) break;
+                    ok = ok && wait_ab(&B->v_full[s], (j / ST) & 1, abort, status);
                     for (int i = row; i < n; i += BM) {
                         const int f = i / ((BN - r0) * 8), e = i - f * (BN - r0) * 8;
                         *reinterpret_cast<uint4*>(sm + L::V + s * L::TILE + f * BOX + r0 * 128 + e * 16) =
@@ -477,6 +480,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
             if constexpr (JOIN) {
                 // the ring is idle once the other slot's last P.V is done too
                 if ((x ? n0 : n1) > 0) ok = ok && wait_ab(&B->o_full[x ^ 1], 0, abort, status);
+                ok = __all_sync(0xffffffffu, ok);
                 if (nx > 0 && ok) {
 #pragma unroll 1
                     for (int cb = 0; cb < D / 64; ++cb) {
@@ -498,6 +502,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                 l = l * w_mine + other.y * w_other;
                 m = M;
             }
+            ok = __all_sync(0xffffffffu, ok);
             // Out through shared memory (this slot's Q, or the unused one, is idle by now): a
             // lane has a row in hand, but rows lie apart in memory, so lanes that store
             // side by side should store one row.

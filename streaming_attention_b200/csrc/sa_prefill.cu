@@ -306,7 +306,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ C
             float m = -INFINITY, l = 0.f;               // m in scaled log2 units
             bool ok = true;
             for (int j = 0; j < my_nkv; ++j) {
-                if (!(ok = wait_ab(&B->s_full[x], j & 1, abort, a.status))) break;
+                if (!(ok = wait_ab_warp(&B->s_full[x], j & 1, abort, a.status))) break;
                 tc::fence_after_sync();
                 uint32_t u32[BN];
 #pragma unroll
@@ -360,7 +360,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ C
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&B->p_full[x]);
             }
-            if (ok && wait_ab(&B->o_full[x], 0, abort, a.status)) {
+            if (ok && wait_ab_warp(&B->o_full[x], 0, abort, a.status)) {
                 tc::fence_after_sync();
                 const float inv = l > 0.f ? 1.f / l : 0.f;
                 const bool store = qrow < P.Sq;
