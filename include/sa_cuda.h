@@ -374,7 +374,8 @@ int sa_attn_decode_noalloc(void* stream, int dtype, const void* q, const void* k
  * stays right as lengths and tables change.  A length that exceeds
  * max_pages * page_size is cut, a page number outside the pool is not
  * accessed (its rows' contribution is undefined), and sa_ctx_synchronize then
- * returns SA_ERR_RANGE.
+ * returns SA_ERR_RANGE.  A device-side wait that expires (SA_ERR_TIMEOUT there)
+ * leaves NaN in the output rows that depend on it.
  *
  * fp32 products run on the tensor cores in the prefill, behind a shared prefix
  * and in decodes with more than four query heads per KV head: each operand as

@@ -119,7 +119,7 @@ struct Joined {
     // The lane's columns of the normalised row, in OT.
     template <typename OT>
     __device__ __forceinline__ void store(OT* dst, int lane) const {
-        const float t = total(), f = t == 0.f ? 0.f : 1.f / t;
+        const float f = row_factor(total());
         dst += lane * V;
         if constexpr (sizeof(OT) == 4) {
 #pragma unroll

@@ -625,8 +625,8 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 const int g = n * 8 + qp + j;
                 if (g >= a.G) continue;
                 if (failed) {
-                    m[n][j] = 0.f;
-                    l[n][j] = nanf("");
+                    m[n][j] = given_up().m;
+                    l[n][j] = given_up().l;
                 }
                 if (ds.kind == TO_OUT) {
                     const float inv = 1.f / l[n][j];     // the pair's query sees its own row at least
@@ -697,8 +697,8 @@ __device__ __forceinline__ void finish_f32(const DecodeArgs& a, Ring* r, const S
             O += y[col] * wt;
         }
         if (failed) {
-            M = 0.f;
-            L = nanf("");
+            M = given_up().m;
+            L = given_up().l;
         }
         if (ds.kind == TO_OUT) {
             static_cast<float*>(a.out)[(long long)b * a.o_stride + (long long)(h * a.G + g) * D + col] = O / L;

@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(FT, (FM == 32 || (FM == 64 && D == 64)) ? 2 : 
             dst = a.part_o + row * D;
         } else {
             dst = a.out + (long long)(tok0 + tk) * a.o_tok + (long long)h * D;
-            f = sum > 0.f ? 1.f / sum : 0.f;
+            f = row_factor(sum);
         }
 #pragma unroll
         for (int c = 0; c < CT; ++c)

@@ -2,6 +2,7 @@
 // touch, and how a batch's tiles are shared out, as plain arithmetic: included
 // by the kernels and compiled with g++ by a CPU test that enumerates it.
 #pragma once
+#include <cmath>
 
 #ifndef __CUDACC__
 #define SA_HD
@@ -87,6 +88,16 @@ SA_HD inline long long append_row(int len, int n, int t, int max_pages, int page
     if (at < 0 || (at >> page_log2) >= max_pages || pos0 + at >= n_pos) return -1;
     return at;
 }
+
+// A query row's softmax state: maximum (log2 units) and sum.  What a row's sums are
+// multiplied by in the end: a row that sees nothing (sum 0) comes out as zeros.
+struct RowState {
+    float m, l;
+};
+SA_HD inline float row_factor(float l) { return l == 0.f ? 0.f : 1.f / l; }
+// The state of a row that a kernel gave up on (an expired wait): the sum stays NaN
+// through every join, whatever the weight of the state there, and so does the output.
+SA_HD inline RowState given_up() { return {0.f, NAN}; }
 
 }  // namespace pg
 }  // namespace sa

@@ -463,24 +463,28 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                 pf::un2(pf::add2(pf::add2(ps[0], ps[1]), pf::add2(ps[2], ps[3])), s0, s1);
                 l += s0 + s1;
             }
-            if (nx > 0) {
-                ok = ok && wait_ab(&B->o_full[x], 0, abort, status);
-                tc::fence_after_sync();
+            if (nx > 0) ok = ok && wait_ab(&B->o_full[x], 0, abort, status);
+            constexpr bool JOIN = ALT && !PREFIX;
+            if constexpr (JOIN) {                                // before the ring is written, below
+                if ((x ? n0 : n1) > 0) ok = ok && wait_ab(&B->o_full[x ^ 1], 0, abort, status);
+            }
+            tc::fence_after_sync();
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
+                m = given_up().m;
+                l = given_up().l;
             }
             // Slots that hold the same rows join their states (those of a prefix are
             // joined with the other splits'): each hands the other's half of O's columns
             // over through the (now idle) K/V ring.  All eight warps come here, after an
             // expired wait too.
-            constexpr bool JOIN = ALT && !PREFIX;
             constexpr int cols = JOIN ? D / 2 : D;
             const int col0 = JOIN ? x * (D / 2) : 0;
             float w_mine = 1.f, w_other = 0.f;
             constexpr int XS = D / 2 + 4;                        // row stride: float4 of eight rows hit all banks
             float* xo = reinterpret_cast<float*>(sm + L::K);     // [2][BM][XS]
             if constexpr (JOIN) {
-                // the ring is idle once the other slot's last P.V is done too
-                if ((x ? n0 : n1) > 0) ok = ok && wait_ab(&B->o_full[x ^ 1], 0, abort, status);
-                ok = __all_sync(0xffffffffu, ok);
+                // the ring is idle: the other slot's last P.V is done too
                 if (nx > 0 && ok) {
 #pragma unroll 1
                     for (int cb = 0; cb < D / 64; ++cb) {
@@ -502,27 +506,30 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                 l = l * w_mine + other.y * w_other;
                 m = M;
             }
-            ok = __all_sync(0xffffffffu, ok);
+            const bool mine = tok < ntok && row < a.tpt * a.G;
+            const float inv = PREFIX ? 1.f : row_factor(l);
+            const float fm = w_mine * inv, fo = w_other * inv;
+            const long long qrow = s_unit.tok0[x] + tok;
+            const int h = kvh * a.G + g;
+            constexpr int ELT = PREFIX ? 4 : 2;
+            unsigned char* dst;                                  // this lane's row, its first column here
+            if constexpr (PREFIX) {
+                const int split = (int)(blockIdx.x / a.units) / a.c.hkv;
+                const long long part = ALT ? 2 * split + x : split;
+                const long long at = (part * a.n_tok + qrow) * a.hq + h;
+                if (mine) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+                dst = reinterpret_cast<unsigned char*>(a.part_o + at * D + col0);
+            } else {
+                dst = static_cast<unsigned char*>(a.out) + (qrow * a.o_tok + (long long)h * D + col0) * 2;
+            }
             // Out through shared memory (this slot's Q, or the unused one, is idle by now): a
             // lane has a row in hand, but rows lie apart in memory, so lanes that store
-            // side by side should store one row.
-            if (ok) {
-                const bool mine = tok < ntok && row < a.tpt * a.G;
-                const float inv = PREFIX ? 1.f : (l > 0.f ? 1.f / l : 0.f);
-                const float fm = w_mine * inv, fo = w_other * inv;
-                const long long qrow = s_unit.tok0[x] + tok;
-                const int h = kvh * a.G + g;
-                constexpr int ELT = PREFIX ? 4 : 2;
-                unsigned char* dst;                              // this lane's row, its first column here
-                if constexpr (PREFIX) {
-                    const int split = (int)(blockIdx.x / a.units) / a.c.hkv;
-                    const long long part = ALT ? 2 * split + x : split;
-                    const long long at = (part * a.n_tok + qrow) * a.hq + h;
-                    if (mine) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
-                    dst = reinterpret_cast<unsigned char*>(a.part_o + at * D + col0);
-                } else {
-                    dst = static_cast<unsigned char*>(a.out) + (qrow * a.o_tok + (long long)h * D + col0) * 2;
-                }
+            // side by side should store one row.  A given-up row is NaN, straight to memory.
+            if (!ok) {
+                if (mine)
+                    for (int i = 0; i < cols * ELT / 16; ++i)
+                        reinterpret_cast<uint4*>(dst)[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+            } else {
                 const uint32_t rows_mine = __ballot_sync(0xffffffffu, mine);
                 constexpr int group = cols < 2 * D / ELT ? cols : 2 * D / ELT;   // columns staged at once: 2 D bytes a row
                 constexpr int lpr = group * ELT / 16;            // 16-byte chunks, and lanes, of a row
