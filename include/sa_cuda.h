@@ -363,7 +363,8 @@ int sa_attn_decode_noalloc(void* stream, int dtype, const void* q, const void* k
  * or 256; page_size 16, 32, 64 or 128; hq / hkv 1..16 (1..8 at d = 256);
  * pointers 16-byte aligned, strides multiples of 16 bytes; n_seqs at most
  * SA_PAGED_MAX_SEQS.  q and out have the cache's element type; scale is
- * positive and finite.  Device pointers only.
+ * positive, at most 2.3586e38 (so that scale * log2(e) is finite in fp32).
+ * Device pointers only.
  *
  * A query at position p sees row j when j <= p and (window = 0, or
  * j > p - window, or j < sinks): a sliding window of `window` rows, its own

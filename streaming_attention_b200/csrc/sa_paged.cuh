@@ -4,6 +4,7 @@
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cmath>
 #include <cstdint>
 
 #include "sa_internal.h"
@@ -15,6 +16,7 @@ namespace sa {
 namespace pg {
 
 constexpr int MAX_GROUP = 16;      // largest hq / hkv
+constexpr float LOG2E = 1.4426950408889634f;      // scores are taken times scale * log2(e)
 
 // The cache as kernels see it: pages of [hkv][page][d] elements.
 struct Cache {
@@ -240,7 +242,8 @@ inline int check_heads(const char* fn, const sa_paged_kv* kv, int hq) {
 }
 
 inline int check_scale(const char* fn, float scale) {
-    SA_CHECK_ARG(scale > 0.f && scale <= 3.0e38f, "%s: scale = %g (want a positive finite number)", fn, (double)scale);
+    SA_CHECK_ARG(scale > 0.f && std::isfinite(scale * LOG2E),
+                 "%s: scale = %g (want a positive number that log2(e) = 1.4427 times is finite in fp32)", fn, (double)scale);
     return SA_OK;
 }
 

@@ -55,7 +55,6 @@ namespace sa {
 namespace pg {
 
 constexpr int STAGES = 3;
-constexpr float LOG2E = 1.4426950408889634f;
 
 enum { JOIN_HERE = 1, JOIN_LATER = 2 };
 struct DecodeArgs {

@@ -30,7 +30,6 @@ namespace sa {
 namespace pg {
 
 constexpr int FN = 64, FT = 256;
-constexpr float F_LOG2E = 1.4426950408889634f;
 
 struct F32Args {
     Cache c;
@@ -388,7 +387,7 @@ int f32_prefill_launch(sa_ctx* ctx, const sa_paged_kv* kv, const float* q, long 
     a.q = q; a.cu_q = cu_q; a.q_tok = q_tok; a.o_tok = o_tok;
     a.n_tok = n_tok; a.hq = hq; a.G = hq / kv->hkv;
     a.window = window; a.sinks = sinks;
-    a.qscale = scale * F_LOG2E;
+    a.qscale = scale * LOG2E;
     a.out = out;
     // 64 rows read K and V half as often as 32; 32 where 64 would leave SMs idle
     const int seqs = std::min(kv->n_seqs, n_tok);
@@ -429,7 +428,7 @@ int f32_prefix_launch(sa_ctx* ctx, const sa_paged_kv* kv, const float* q, long l
     a.n_tok = kv->n_seqs; a.hq = hq; a.G = hq / kv->hkv;
     const int fm = f32_prefix_rows(kv, a.G);
     a.tpt = fm / a.G;
-    a.qscale = scale * F_LOG2E;
+    a.qscale = scale * LOG2E;
     a.prefix_table = prefix_table; a.prefix_len = prefix_len;
     a.n_split = n_split;
     a.units = (kv->n_seqs + a.tpt - 1) / a.tpt;

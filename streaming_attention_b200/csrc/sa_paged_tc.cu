@@ -636,7 +636,7 @@ int tc_prefill_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long lo
     a.cu_q = cu_q;
     a.window = window;
     a.sinks = sinks;
-    a.sl2 = scale * pf::LOG2E;
+    a.sl2 = scale * LOG2E;
     a.out = out;
     a.o_tok = o_tok;
     // Every sequence's last unit may be partly filled.  Few units leave SMs idle:
@@ -669,7 +669,7 @@ int tc_prefix_launch(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long lon
     CUtensorMap mq, mk, mv;
     SA_RC_TRY(tc_maps(kv, q, q_tok, kv->n_seqs, hq, &a, &mq, &mk, &mv));
     a.c = make_cache(ctx, kv);
-    a.sl2 = scale * pf::LOG2E;
+    a.sl2 = scale * LOG2E;
     a.prefix_table = prefix_table;
     a.prefix_len = prefix_len;
     a.n_split = n_split;
