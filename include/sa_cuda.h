@@ -381,7 +381,13 @@ int sa_attn_decode_noalloc(void* stream, int dtype, const void* q, const void* k
  * fp32 products run on the tensor cores in the prefill, behind a shared prefix
  * and in decodes with more than four query heads per KV head: each operand as
  * the sum of two tf32 numbers, which keeps fp32's precision for magnitudes from
- * 2^-100 to 2^127 (smaller ones lose bits, larger ones may overflow).
+ * 2^-100 on (smaller ones lose bits).
+ *
+ * Magnitudes: values are summed before the division by the sum of the weights,
+ * so max |v| times the number of rows that a query sees is at most 2^127 in
+ * fp32, 2^118 in bf16 (whose weights may exceed 1, up to 2^9); the scores,
+ * scale * q.k, are at most 2^126 in fp32, 2^24 in bf16, and so are scale * q
+ * and the partial sums.  Beyond, a result may be infinite or NaN.
  *
  * Workspaces are the caller's (256-byte aligned device memory); calls that may
  * run at the same time, captured ones included, need workspaces of their own.

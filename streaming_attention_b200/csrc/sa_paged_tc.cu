@@ -410,7 +410,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                                                        pf::bits_below(first - w * 32));
                 }
                 // the running maximum moves, and O is rescaled, only when a row's
-                // scores outgrow it by 2^8 (the last P.V completed before S came)
+                // scores outgrow it by 2^8 (the last P.V completed before S came):
+                // weights reach 2^8, 2^9 where the maximum itself is rounded (scores of 2^24)
                 const float mxs = pf::row_max3(sc) * sl2;
                 const bool need = mxs > m + pf::RESCALE_THRESHOLD;
                 if (__any_sync(0xffffffffu, need)) {
