@@ -464,7 +464,10 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
                 pf::un2(pf::add2(pf::add2(ps[0], ps[1]), pf::add2(ps[2], ps[3])), s0, s1);
                 l += s0 + s1;
             }
+            // A slot without a tile beside one with tiles has its Q on the way all the same: the
+            // rows' zeros are staged where it lands.
             if (nx > 0) ok = ok && wait_ab(&B->o_full[x], 0, abort, status);
+            else if (!ALT && n_kv > 0) ok = ok && wait_ab(&B->q_full, 0, abort, status);
             constexpr bool JOIN = ALT && !PREFIX;
             if constexpr (JOIN) {                                // before the ring is written, below
                 if ((x ? n0 : n1) > 0) ok = ok && wait_ab(&B->o_full[x ^ 1], 0, abort, status);

@@ -80,3 +80,26 @@ def test_prefill_variants(case):
         ref = attend(q[r], pool.k[b], pool.v[b], list(range(n - new[b], n)), d ** -0.5, window, sinks)
         off = (out[r].double() - ref).abs() - bound("bf16", ref, n)
         assert not off.numel() or off.max().item() <= 0, (b, off.max().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(16, 8, 128), (12, 6, 64)])
+def test_a_slot_before_the_first_row_beside_one_with_rows(hq, hkv, d):
+    """A chunk longer than its sequence: the CTA that holds row 0 has a first slot of tokens that see nothing, whose
+    queries are loaded all the same; they get zeros, and the second slot its results."""
+    import streaming_attention_b200 as sa
+    new, n = 2600, 985
+    case = ([new], [0], hq, hkv, d, 16, 0, 0)
+    per, first = 128 // (hq // hkv), new - n                     # tokens of a slot; the token at row 0
+    assert first // per % 2 == 1 and first % per
+    with sa.Context(0) as ctx:
+        assert _two_slots(case, ctx.num_sms)
+        pool = mark(Pool([n], hkv, d, 16, "bf16", seed=5))
+        q = pool.q(new, hq, SPREAD)
+        cu = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+        for _ in range(20):
+            out = sa.attn_paged_prefill(q.cuda(), pool.kp, pool.vp, pool.table, pool.kv_lens, cu, d ** -0.5, ctx=ctx)
+            ctx.synchronize()
+            assert (out[:first] == 0).all()
+    ref = attend(q[first:], pool.k[0], pool.v[0], list(range(n)), d ** -0.5)
+    assert ((out[first:].double().cpu() - ref).abs() <= bound("bf16", ref, n)).all()
