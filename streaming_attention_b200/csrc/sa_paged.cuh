@@ -144,18 +144,19 @@ struct SeqUnit {
 // Tokens of a sequence; a range outside the token tensors is reported and counts
 // as none.
 __device__ __forceinline__ int seq_tokens(const Cache& c, int c0, int c1, int n_tok) {
-    if (c0 >= 0 && c1 <= n_tok && c1 >= c0) return c1 - c0;
+    const int n = token_count(c0, c1, n_tok);
+    if (n >= 0) return n;
     atomicExch(c.bad, SA_STATUS_BAD_INDEX);
     return 0;
 }
 // Unit total - 1 - back of the batch, by the whole block (scan: THREADS / 32
-// ints); false when there is none.
+// numbers); false when there is none.
 template <int THREADS>
-__device__ bool find_seq_unit(const Cache& c, const int* cu_q, int n_tok, int per, int back, SeqUnit* s, int* scan) {
+__device__ bool find_seq_unit(const Cache& c, const int* cu_q, int n_tok, int per, int back, SeqUnit* s, unsigned* scan) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int run = (c.n_seqs + THREADS - 1) / THREADS;
     const int b0 = min(c.n_seqs, tid * run), b1 = min(c.n_seqs, b0 + run);
-    int mine = 0;
+    unsigned mine = 0;
     const int len0 = b0 < b1 ? seq_len(c, b0) : 0;       // in flight with cu_q: most runs are one sequence
     for (int b = b0; b < b1; b += 8) {                   // eight loads in flight where runs are long
         int cu[9];
@@ -163,38 +164,33 @@ __device__ bool find_seq_unit(const Cache& c, const int* cu_q, int n_tok, int pe
         for (int u = 0; u < 9; ++u) cu[u] = cu_q[min(b + u, b1)];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (b + u < b1) mine += (seq_tokens(c, cu[u], cu[u + 1], n_tok) + per - 1) / per;
+            if (b + u < b1) mine = add_units(mine, unit_count(seq_tokens(c, cu[u], cu[u + 1], n_tok), per), THREADS);
     }
-    int inc = mine;
+    unsigned inc = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, inc, off);
+        const unsigned up = __shfl_up_sync(0xffffffffu, inc, off);
         if (lane >= off) inc += up;
     }
     if (lane == 31) scan[warp] = inc;
     __syncthreads();
-    int before = 0, total = 0;
+    unsigned before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) before += scan[w];
         total += scan[w];
     }
-    const int want = total - 1 - back;
-    if (want < 0) return false;
-    int at = before + inc - mine;
-    if (want >= at && want < at + mine)
-        for (int b = b0; b < b1; ++b) {
-            const int first = cu_q[b], n = seq_tokens(c, first, cu_q[b + 1], n_tok), u = (n + per - 1) / per;
-            if (want < at + u) {
-                s->b = b;
-                s->unit = want - at;
-                s->first = first;
-                s->tokens = n;
-                s->len = b == b0 ? len0 : seq_len(c, b);
-                break;
-            }
-            at += u;
-        }
+    if ((unsigned)back >= total) return false;
+    const unsigned want = total - 1u - (unsigned)back;
+    unsigned at = before + inc - mine;
+    if (want >= at && want - at < mine) {
+        const int b = unit_sequence(cu_q, b0, b1, n_tok, per, want, &at);
+        s->b = b;
+        s->unit = (int)(want - at);
+        s->first = cu_q[b];
+        s->tokens = cu_q[b + 1] - cu_q[b];
+        s->len = b == b0 ? len0 : seq_len(c, b);
+    }
     __syncthreads();
     return true;
 }

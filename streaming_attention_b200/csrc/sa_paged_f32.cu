@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(FT, (FM == 32 || (FM == 64 && D == 64)) ? 2 : 
     constexpr int NG = NT < 4 ? NT : 4, CG = CT < 4 ? CT : 4;    // blocks whose products interleave
     extern __shared__ __align__(16) float smf[];
     __shared__ SeqUnit s_seq;
-    __shared__ int s_scan[FT / 32];
+    __shared__ unsigned s_scan[FT / 32];
     float *sQ = smf + L::Q, *sK = smf + L::K, *sV = smf + L::V, *sP = smf + L::P, *sX = smf + L::X;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int wm = warp % L::WM, wn = warp / L::WM;      // the warp's 16 MR rows; its keys and columns

@@ -81,6 +81,28 @@ SA_HD inline int share_of(long long tile, long long total, long long n) {
     return (int)(((tile + 1) * n - 1) / total);
 }
 
+// Tokens [c0, c1) of a sequence, -1 for a range outside the n_tok of the token tensors;
+// the units of up to `per` tokens that they are cut into.
+SA_HD inline int token_count(int c0, int c1, int n_tok) { return c0 >= 0 && c1 <= n_tok && c1 >= c0 ? c1 - c0 : -1; }
+SA_HD inline unsigned unit_count(int tokens, int per) { return tokens > 0 ? (unsigned)(tokens - 1) / per + 1u : 0u; }
+// Adds to the units of a thread's run of sequences.  Ranges of a wrong cu_q may overlap,
+// so a run counts for what keeps the block's sum in 32 bits; a right one's units, of rows
+// that lie in memory, stay far below (some 2^23 at 180 GB).
+SA_HD inline unsigned add_units(unsigned run, unsigned units, unsigned threads) {
+    const unsigned cap = 0xffffffffu / threads;
+    return run + units < cap ? run + units : cap;
+}
+// The sequence of [b0, b1), whose units begin at number `at`, that unit `want` >= at is in,
+// and the number of that sequence's first unit; -1: none.
+SA_HD inline int unit_sequence(const int* cu_q, int b0, int b1, int n_tok, int per, unsigned want, unsigned* at) {
+    for (int b = b0; b < b1; ++b) {
+        const unsigned u = unit_count(token_count(cu_q[b], cu_q[b + 1], n_tok), per);
+        if (want - *at < u) return b;
+        *at += u;
+    }
+    return -1;
+}
+
 // The row of token t (of n) of a sequence of `len` rows, -1 if the cache has
 // no such row or the angle table no such position.
 SA_HD inline long long append_row(int len, int n, int t, int max_pages, int page_log2, long long pos0, long long n_pos) {

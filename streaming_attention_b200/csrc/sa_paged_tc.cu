@@ -111,7 +111,7 @@ struct Unit {
 // sequence see the most rows: they start first).  A unit is the tokens of two
 // slots, or of one tile that both slots hold (ALT).
 template <bool ALT>
-__device__ bool find_prefill_unit(const TcArgs& a, Unit* s, SeqUnit* su, int* scan) {
+__device__ bool find_prefill_unit(const TcArgs& a, Unit* s, SeqUnit* su, unsigned* scan) {
     const int per = ALT ? a.tpt : 2 * a.tpt;
     if (!find_seq_unit<TC_THREADS>(a.c, a.cu_q, a.n_tok, per, blockIdx.x / a.c.hkv, su, scan)) return false;
     if (threadIdx.x == 0) {
@@ -177,7 +177,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ 
     extern __shared__ unsigned char smem_raw[];
     __shared__ Unit s_unit;
     __shared__ SeqUnit s_seq;
-    __shared__ int s_scan[TC_THREADS / 32];
+    __shared__ unsigned s_scan[TC_THREADS / 32];
     __shared__ float2 s_ml[2][BM];
     const uint32_t raw = smem_u32(smem_raw);
     unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
