@@ -103,11 +103,12 @@ SA_HD inline int unit_sequence(const int* cu_q, int b0, int b1, int n_tok, int p
     return -1;
 }
 
-// The row of token t (of n) of a sequence of `len` rows, -1 if the cache has
-// no such row or the angle table no such position.
+// The row of token t (of n) of a sequence of `len` rows, -1 if the sequence has
+// no such token (a wrong cu_q), the cache no such row or the angle table no such
+// position.
 SA_HD inline long long append_row(int len, int n, int t, int max_pages, int page_log2, long long pos0, long long n_pos) {
     const long long at = (long long)len - n + t;
-    if (at < 0 || (at >> page_log2) >= max_pages || pos0 + at >= n_pos) return -1;
+    if (t < 0 || t >= n || at < 0 || (at >> page_log2) >= max_pages || pos0 + at >= n_pos) return -1;
     return at;
 }
 
