@@ -98,7 +98,7 @@ def _cache(k_pages, v_pages, block_table, kv_lens):
     code = _code(k_pages, "pages")
     n_pages, hkv, page, d = shape
     for s in (stride, v_pages.stride()):
-        if s[3] != 1 or s[2] != d or s[1] != page * d or (n_pages > 1 and s[0] != stride[0]):
+        if s[3] != 1 or s[2] != d or (hkv > 1 and s[1] != page * d) or (n_pages > 1 and s[0] != stride[0]):
             raise ValueError(f"pages: [hkv, page_size, d] of a page must be contiguous, k and v alike (strides {s})")
     if block_table.dim() != 2 or block_table.dtype is not _torch.int32 or block_table.get_device() != dev:
         raise ValueError(f"block_table: want int32 [n_seqs, max_pages] on GPU {dev}, "
