@@ -134,6 +134,14 @@ def _size(key, size_fn, *args) -> int:
     return n
 
 
+def _capturing(dev: int) -> bool:
+    """Whether torch's current stream of that GPU, which need not be the current one, is being captured."""
+    if _torch._C._cuda_getDevice() == dev:
+        return _torch._C._cuda_isCurrentStreamCapturing()
+    with _torch.cuda.device(dev):
+        return _torch._C._cuda_isCurrentStreamCapturing()
+
+
 def _workspace(ctx: Context, dev: int, n: int):
     """A decode's workspace, its head zero; a captured call has its own.
 
@@ -142,7 +150,7 @@ def _workspace(ctx: Context, dev: int, n: int):
     another) do not: they have a context each, and a call may be several launches,
     which pass states through the workspace while another call's lie between them.
     """
-    if _torch._C._cuda_isCurrentStreamCapturing():
+    if _capturing(dev):
         ws = _torch.empty(n, dtype=_torch.uint8, device=dev)
         ws[:SA_PAGED_ZERO_BYTES].zero_()
         return ws

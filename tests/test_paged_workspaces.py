@@ -1,5 +1,6 @@
 """The workspaces that the paged operators keep: one per context and stream, so
 that threads which share a stream, with a context each, do not meet in one."""
+import contextlib
 import threading
 import types
 
@@ -18,14 +19,23 @@ class _Ctx:
 def paged(monkeypatch):
     """The module with torch's CUDA calls replaced by ones that work on the CPU; ``state`` sets stream and capture."""
     from streaming_attention_b200 import paged
-    state = types.SimpleNamespace(stream=7, capturing=False)
+    state = types.SimpleNamespace(stream=7, capturing=False, device=0, other_capturing=False)
+
+    @contextlib.contextmanager
+    def device(dev):
+        before, state.device = state.device, dev
+        yield
+        state.device = before
+
     fake = types.SimpleNamespace(
         uint8=torch.uint8,
         zeros=lambda n, dtype, device: torch.zeros(n, dtype=dtype),
         empty=lambda n, dtype, device: torch.full((n,), 9, dtype=dtype),
-        _C=types.SimpleNamespace(_cuda_isCurrentStreamCapturing=lambda: state.capturing,
+        cuda=types.SimpleNamespace(device=device),
+        _C=types.SimpleNamespace(_cuda_isCurrentStreamCapturing=lambda: state.capturing if state.device == 0
+                                 else state.other_capturing,
                                  _cuda_getCurrentRawStream=lambda dev: state.stream,
-                                 _cuda_getDevice=lambda: 0))
+                                 _cuda_getDevice=lambda: state.device))
     monkeypatch.setattr(paged, "_torch", fake)
     paged.state = state
     return paged
@@ -53,6 +63,18 @@ def test_a_captured_call_has_its_own_with_a_zero_head(paged):
     assert not one[:4096].any() and not two[:4096].any()
     paged.state.capturing = False
     assert paged._workspace(a, 0, 9000) is kept
+
+
+def test_the_capture_is_looked_for_on_the_pages_gpu(paged):
+    """Pages on GPU 0 while GPU 1 is the current one: whose stream is captured decides."""
+    a = _Ctx()
+    kept = paged._workspace(a, 0, 9000)
+    paged.state.device, paged.state.other_capturing = 1, True
+    assert paged._workspace(a, 0, 9000) is kept                 # GPU 1's capture is not this call's
+    paged.state.other_capturing, paged.state.capturing = False, True
+    own = paged._workspace(a, 0, 9000)
+    assert own.data_ptr() != kept.data_ptr() and not own[:4096].any()
+    assert paged.state.device == 1
 
 
 @pytest.mark.gpu
