@@ -447,7 +447,8 @@ int sa_paged_append(sa_ctx* ctx, const sa_paged_kv* kv, int x_dtype, const void*
 /*
  * One query token per sequence, at its last row: q, out [n_seqs, hq, d] with
  * q_stride / o_stride elements between sequences.  Softmax and sums in fp32;
- * bf16 products take the softmax weights in bf16 (as the output is).
+ * bf16 products take each softmax weight as the sum of two bf16 numbers (2^-16
+ * of it left out), so the output's rounding is the one that shows.
  */
 int sa_attn_paged_decode_workspace(sa_ctx* ctx, const sa_paged_kv* kv, int hq, size_t* bytes);
 int sa_attn_paged_decode(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_stride, int hq, int window,
@@ -458,8 +459,10 @@ int sa_attn_paged_decode(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long
  * A ragged batch of prompt chunks: q, out [n_tokens, hq, d] (token strides in
  * elements), tokens cu_q[b] .. cu_q[b+1] - 1 the last ones of sequence b
  * (token t of n at position kv_lens[b] - n + t), whose keys and values are in
- * the pages.  Causal, with the window above.  bf16 on the tensor cores
- * (softmax weights in bf16, sums in fp32), fp32 there too (above).  d 64 or 128.
+ * the pages.  Causal, with the window above.  bf16 on the tensor cores, fp32
+ * there too (above).  In bf16 the softmax weights are rounded to bf16 for the
+ * product with the values (their sum is not): 2^-8 of sum w |v| beside the
+ * output's own rounding.  d 64 or 128.
  * Rows behind the last sequence are left as they were.
  */
 int sa_attn_paged_prefill(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, long long q_tok_stride, int n_tokens,
@@ -472,7 +475,8 @@ int sa_attn_paged_prefill(sa_ctx* ctx, const sa_paged_kv* kv, const void* q, lon
  * the pages of the prefix_len shared rows (device memory, ceil(prefix_len /
  * page_size) entries); kv's block table and lengths are those of the own rows
  * alone (a length may be 0).  The prefix is read once for the whole batch.
- * d 64 or 128.
+ * Weights of the prefix's rows are rounded as in the prefill, those of the own
+ * rows as in the decode.  d 64 or 128.
  */
 int sa_attn_paged_decode_prefix_workspace(sa_ctx* ctx, const sa_paged_kv* kv, int hq, int prefix_len,
                                           size_t* bytes);

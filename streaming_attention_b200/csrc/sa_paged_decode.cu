@@ -27,7 +27,11 @@
 //    P^T turns from accumulator to operand layout by movmatrix, without shared
 //    memory.  (tcgen05 wants M = 128 rows of A from shared memory and its
 //    result in TMEM; at 4 G FLOP per 4 bytes the tensor rate is not what binds.)
-//    P is rounded to bf16 for the product (as the output is), its sum is not.
+//    P enters the product as the sum of two bf16 numbers: HBM binds, so the second
+//    product costs nothing over long rows (64 sequences, below: 172.8 us, 173.0 with
+//    one), 0.1-1 us where short ones leave it in the chain of latencies (1024
+//    sequences of 30 rows: 62.7, 61.7).  Against 64 bits 1.65e-3, the output's
+//    rounding alone; with one 1.95e-3.
 //  * fp32, up to four heads per KV head: four warps per group of at most HG heads, on
 //    FMAs, an 8-lane group per row; scores, weights and sums in fp32.
 //  * fp32, more heads: on the tensor cores, three tf32 products for one of fp32.
@@ -213,6 +217,10 @@ __device__ __forceinline__ long long share_slot(const Shares& x, int p) { return
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+// What the pair h = pack2(a, b) leaves of a and b.
+__device__ __forceinline__ uint32_t rest2(uint32_t h, float a, float b) {
+    return pack2(a - __uint_as_float(h << 16), b - __uint_as_float(h & 0xffff0000u));
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -547,7 +555,7 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                         vmask[e] = (t.sees(j0 + qp + 8 * e) ? 0x0000ffffu : 0u) |
                                    (t.sees(j0 + qp + 1 + 8 * e) ? 0xffff0000u : 0u);
                 }
-                uint32_t pf[NT][2];
+                uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float mx0 = fmaxf(sc[n][0], sc[n][2]), mx1 = fmaxf(sc[n][1], sc[n][3]);
@@ -577,8 +585,11 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     const float p2 = ex2(fmaf(sc[n][2], a.qscale, z0)), p3 = ex2(fmaf(sc[n][3], a.qscale, z1));
                     l[n][0] += p0 + p2;
                     l[n][1] += p1 + p3;
-                    pf[n][0] = movm(pack2(p0, p1));
-                    pf[n][1] = movm(pack2(p2, p3));
+                    const uint32_t h0 = pack2(p0, p1), h1 = pack2(p2, p3);
+                    ph[n][0] = movm(h0);
+                    ph[n][1] = movm(h1);
+                    pl[n][0] = movm(rest2(h0, p0, p1));
+                    pl[n][1] = movm(rest2(h1, p2, p3));
                 }
                 const int vrow = r0 + ((lane >> 4) << 3) + (lane & 7);
 #pragma unroll
@@ -593,7 +604,10 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                         vf[3] &= vmask[1];
                     }
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma16816(o[n][d], vf, pf[n][0], pf[n][1]);
+                    for (int n = 0; n < NT; ++n) {
+                        mma16816(o[n][d], vf, ph[n][0], ph[n][1]);
+                        mma16816(o[n][d], vf, pl[n][0], pl[n][1]);
+                    }
                 }
             }
             __syncwarp();
