@@ -29,8 +29,8 @@
 //    result in TMEM; at 4 G FLOP per 4 bytes the tensor rate is not what binds.)
 //    P enters the product as the sum of two bf16 numbers: HBM binds, so the second
 //    product costs nothing over long rows (64 sequences, below: 172.8 us, 173.0 with
-//    one), 0.1-1 us where short ones leave it in the chain of latencies (1024
-//    sequences of 30 rows: 62.7, 61.7).  Against 64 bits 1.65e-3, the output's
+//    one), and 0.1-0.8 us where short ones leave it in the chain of latencies (1024
+//    sequences of 30 rows: 61.9, 61.1).  Against 64 bits 1.65e-3, the output's
 //    rounding alone; with one 1.95e-3.
 //  * fp32, up to four heads per KV head: four warps per group of at most HG heads, on
 //    FMAs, an 8-lane group per row; scores, weights and sums in fp32.
@@ -248,24 +248,25 @@ struct Ring {
     uint64_t full[STAGES], empty[STAGES];
     long long scan[40];
     Share share;
-    int issued, consumed;
+    int issued;
     int failed;              // a consumer's wait expired: what follows is NaN
     int last;                // this CTA handed in a pair's last share
 };
 
-// A wait of a whole (converged) warp: its lanes look at the barrier and the clock
-// one by one, and go on together or give up together.
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
+// A consumer lane's wait for tile `it` of its share; one that expires is noted, and the
+// lane goes on without further waits over whatever the ring holds: the warp stays
+// together at its shuffles and products without a vote per tile (1024 sequences of 30
+// rows: 61.9 us, 62.7 with one), meets every barrier, and hands every share in as NaN.
+__device__ __forceinline__ void consume_wait(Ring* r, int it, bool& ok, int* status) {
+    if (ok && !mbar_wait(r->full + it % STAGES, (it / STAGES) & 1, status)) {
+        ok = false;
+        r->failed = 1;
+    }
 }
-// A consumer warp's wait for tile `it` of its share; the first that expires is
-// noted, and no further one is waited for.
-__device__ __forceinline__ bool consume_wait(Ring* r, int it, bool& ok, int* status) {
-    if (!ok) return false;
-    if ((ok = mbar_wait_warp(r->full + it % STAGES, (it / STAGES) & 1, status))) return true;
-    atomicMin(&r->consumed, it);
-    r->failed = 1;
-    return false;
+// The stage is free again; after an expired wait it is not: its copy may be on its way.
+__device__ __forceinline__ void consumed(Ring* r, int s, bool ok, int lane) {
+    __syncwarp();
+    if (lane == 0 && ok) mbar_arrive(r->empty + s);
 }
 
 // For a kernel that joins the states later: where it finds a pair's.
@@ -348,7 +349,8 @@ __device__ __forceinline__ void produce(const CUtensorMap* tk, const CUtensorMap
         w.next(a, TK);
         if (it + 1 < n) entry = lookup(w);
         const int s = it % STAGES;
-        if (it >= STAGES && !mbar_wait_warp(r->empty + s, ((it / STAGES) & 1) ^ 1, a.c.status)) break;
+        const bool free = it < STAGES || mbar_wait(r->empty + s, ((it / STAGES) & 1) ^ 1, a.c.status);
+        if (!__all_sync(0xffffffffu, free)) break;       // the lanes give up together
         const unsigned got = __ballot_sync(0xffffffffu, page_id >= 0);
         const uint32_t bytes = (uint32_t)(rows * D * Z::ELT);
         if (lane == 0) mbar_arrive_expect_tx(r->full + s, 2 * __popc(got) * bytes);
@@ -383,8 +385,9 @@ __device__ __forceinline__ void produce(const CUtensorMap* tk, const CUtensorMap
 // it leaves.
 __device__ __forceinline__ void drain(Ring* r) {
     __syncthreads();
-    if (threadIdx.x == 0)
-        for (int it = r->consumed; it < r->issued; ++it) mbar_wait(r->full + it % STAGES, (it / STAGES) & 1, nullptr);
+    if (threadIdx.x == 0 && r->failed)
+        for (int it = max(0, r->issued - STAGES); it < r->issued; ++it)
+            mbar_wait(r->full + it % STAGES, (it / STAGES) & 1, nullptr);
     __syncthreads();
 }
 
@@ -462,7 +465,6 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         leave(a);
         return;
     }
-    if (tid == 0) r.consumed = sh.count;
     Walk w;
     w.b = sh.b; w.h = sh.h; w.i = sh.i; w.left = sh.count;
     w.t = tiles_of(a, seq_len(a.c, w.b), TK);
@@ -492,8 +494,6 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
     };
     load_q(w.b, w.h);
-    // After an expired wait the walk goes on without its tiles, so that the warps
-    // meet at every barrier and every share is handed in (as NaN).
     int it = 0;
     bool ok = true;
     while (w.left > 0) {
@@ -514,10 +514,7 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
         for (int i = i0; i < i1; ++i, ++it) {
             const int s = it % STAGES;
-            if (!consume_wait(&r, it, ok, a.c.status)) {
-                w.next(a, TK);
-                continue;
-            }
+            consume_wait(&r, it, ok, a.c.status);
             const uint32_t ks = sbuf + s * Z::STAGE_BYTES, vs = ks + Z::STAGE_BYTES / 2;
             const int row0 = t.row0(i, TK);
 #pragma unroll
@@ -610,8 +607,7 @@ decode_bf16_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(r.empty + s);
+            consumed(&r, s, ok, lane);
             w.next(a, TK);
         }
         if (w.left > 0) load_q(w.b, w.h);
@@ -756,7 +752,6 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
         leave(a);
         return;
     }
-    if (tid == 0) r.consumed = sh.count;
     Walk w;
     w.b = sh.b; w.h = sh.h; w.i = sh.i; w.left = sh.count;
     w.t = tiles_of(a, seq_len(a.c, w.b), TK);
@@ -805,10 +800,7 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
         }
         for (int i = i0; i < i1; ++i, ++it) {
             const int s = it % STAGES;
-            if (!consume_wait(&r, it, ok, a.c.status)) {
-                w.next(a, TK);
-                continue;
-            }
+            consume_wait(&r, it, ok, a.c.status);
             const unsigned char* ks = buf + s * Z::STAGE_BYTES;
             const unsigned char* vs = ks + Z::STAGE_BYTES / 2;
             const int row0 = t.row0(i, TK);
@@ -872,8 +864,7 @@ decode_f32_kernel(const __grid_constant__ DecodeArgs a) {
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(r.empty + s);
+            consumed(&r, s, ok, lane);
             w.next(a, TK);
         }
         const bool whole = i0 == 0 && i1 == t.n;
@@ -955,7 +946,6 @@ decode_f32_heads_kernel(const __grid_constant__ DecodeArgs a) {
         leave(a);
         return;
     }
-    if (tid == 0) r.consumed = sh.count;
     Walk w;
     w.b = sh.b; w.h = sh.h; w.i = sh.i; w.left = sh.count;
     w.t = tiles_of(a, seq_len(a.c, w.b), TK);
@@ -1018,10 +1008,7 @@ decode_f32_heads_kernel(const __grid_constant__ DecodeArgs a) {
             for (int e = 0; e < 2 * MH; ++e) o[c][e] = 0.f;
         for (int i = i0; i < i1; ++i, ++it) {
             const int s = it % STAGES;
-            if (!consume_wait(&r, it, ok, a.c.status)) {
-                w.next(a, TK);
-                continue;
-            }
+            consume_wait(&r, it, ok, a.c.status);
             const unsigned char* ks = buf + s * Z::STAGE_BYTES + warp * F::RW * (D * 4);
             const unsigned char* vs = ks + Z::STAGE_BYTES / 2;
             const int row0 = t.row0(i, TK) + warp * F::RW;
@@ -1153,8 +1140,7 @@ decode_f32_heads_kernel(const __grid_constant__ DecodeArgs a) {
 #pragma unroll
                     for (int e = 0; e < 2 * MH; ++e) o[c + u][e] += d[u][e];
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(r.empty + s);
+            consumed(&r, s, ok, lane);
             w.next(a, TK);
         }
         const bool whole = i0 == 0 && i1 == t.n;
