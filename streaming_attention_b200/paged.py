@@ -55,11 +55,14 @@ def _code(x, what: str) -> int:
     raise TypeError(f"{what}: dtype {x.dtype} (want float32 or bfloat16)")
 
 
-def _int(x: int, what: str) -> int:
-    """x as a C int (ctypes cuts what does not fit)."""
-    if not -0x80000000 <= x <= 0x7fffffff:
-        raise ValueError(f"{what}: {x} does not fit an int")
-    return x
+_INT_MAX = 0x7fffffff
+
+
+def _ints(**numbers: int) -> None:
+    """Refuses numbers that do not fit a C int (ctypes cuts them); negative ones that do are the library's to refuse."""
+    for what, x in numbers.items():
+        if not -0x80000000 <= x <= _INT_MAX:
+            raise ValueError(f"{what}: {x} does not fit an int")
 
 
 def _index(x, what: str, n: int, dev: int) -> int:
@@ -164,8 +167,7 @@ def _workspace(ctx: Context, dev: int, n: int):
 def rope_table(theta: float, rotary_dim: int, n_pos: int, device="cuda", ctx: Context | None = None):
     """(cos, sin), each [n_pos, rotary_dim // 2] fp32, of the angles p * theta^(-2i / rotary_dim) (sa_rope_table)."""
     torch = _load()
-    _int(n_pos, "n_pos")
-    _int(rotary_dim, "rotary_dim")
+    _ints(n_pos=n_pos, rotary_dim=rotary_dim)
     device = torch.device(device)
     dev = device.index if device.index is not None else torch.cuda.current_device()
     cos = torch.empty(n_pos, rotary_dim // 2, dtype=torch.float32, device=torch.device("cuda", dev))
@@ -185,7 +187,8 @@ def paged_append(k, v, k_pages, v_pages, block_table, kv_lens, cu_q=None, q=None
     k, v and q share a dtype (fp32 or bf16), any row stride.  Returns the
     rotated queries in the pages' dtype (None without q).
     """
-    _int(pos0, "pos0")
+    if not 0 <= pos0 <= _INT_MAX:
+        _ints(pos0=pos0)
     kv, dev, dt, _, hkv, d, _, n_seqs = _cache(k_pages, v_pages, block_table, kv_lens)
     n, xdt = k.shape[0], k.dtype
     ks, vs = _rows(k, "k", n, hkv, d, dev, xdt), _rows(v, "v", n, hkv, d, dev, xdt)
@@ -207,7 +210,8 @@ def paged_append(k, v, k_pages, v_pages, block_table, kv_lens, cu_q=None, q=None
     if rope is not None:
         cos, sin = rope
         n_pos, half = cos.shape
-        _int(n_pos, "rope: positions")
+        if n_pos > _INT_MAX:
+            _ints(rope_positions=n_pos)
         rot = 2 * half
         for x in rope:
             if x.dtype is not _torch.float32 or x.shape != cos.shape or x.get_device() != dev or not x.is_contiguous():
@@ -227,8 +231,8 @@ def attn_paged_decode(q, k_pages, v_pages, block_table, kv_lens, scale: float, w
     and the first ``sinks`` rows.  Returns [n_seqs, hq, d] in q's dtype; a
     sequence of length 0 gets zeros.
     """
-    _int(window, "window")
-    _int(sinks, "sinks")
+    if not (0 <= window <= _INT_MAX and 0 <= sinks <= _INT_MAX):
+        _ints(window=window, sinks=sinks)
     kv, dev, dt, code, hkv, d, _, n_seqs = _cache(k_pages, v_pages, block_table, kv_lens)
     qs = _rows(q, "q", n_seqs, None, d, dev, dt)
     hq = q.shape[1]
@@ -253,8 +257,8 @@ def attn_paged_prefill(q, k_pages, v_pages, block_table, kv_lens, cu_q, scale: f
     attn_paged_decode.  Returns [n_tokens, hq, d]; rows behind the last
     sequence are not written.
     """
-    _int(window, "window")
-    _int(sinks, "sinks")
+    if not (0 <= window <= _INT_MAX and 0 <= sinks <= _INT_MAX):
+        _ints(window=window, sinks=sinks)
     kv, dev, dt, _, _, d, _, n_seqs = _cache(k_pages, v_pages, block_table, kv_lens)
     n = q.shape[0]
     qs = _rows(q, "q", n, None, d, dev, dt)
@@ -278,7 +282,8 @@ def attn_paged_decode_prefix(q, k_pages, v_pages, prefix_table, prefix_len: int,
     length may be 0).  q [n_seqs, hq, d] sees all of both.  d 64 or 128.
     Returns [n_seqs, hq, d].
     """
-    _int(prefix_len, "prefix_len")
+    if not 0 <= prefix_len <= _INT_MAX:
+        _ints(prefix_len=prefix_len)
     kv, dev, dt, code, hkv, d, page, n_seqs = _cache(k_pages, v_pages, block_table, kv_lens)
     qs = _rows(q, "q", n_seqs, None, d, dev, dt)
     hq = q.shape[1]
