@@ -17,8 +17,11 @@
 // softmax between its products; small calls by the latency of few dependent tiles.
 // Measured: 16 sequences behind 4001 rows, 16/8 heads of 128: 22.9 us for the
 // prefix (42 on FMAs); three chunks of up to 300 tokens, 8/4 heads of 64, window
-// 129: 21.8 us (29); 4096 tokens, 16/8 heads of 128: 1260 us, 55 TFLOP/s of 97 (45
-// with 64 rows); errors against 64 bits 2e-7.
+// 129: 21.8 us (29); 4096 tokens, 16/8 heads of 128: 1260 us, 55 TFLOP/s (45 with 64
+// rows) of the 97 that three products of mma.sync give -- tcgen05's kind::tf32, half
+// of bf16's rate, would give 282; errors against 64 bits 2e-7.  A CTA walks over all
+// keys of its rows, so few tokens after a long cache leave SMs idle: 16 tokens, 32768
+// rows: 2.2 ms.
 #include <algorithm>
 #include <cmath>
 

@@ -38,8 +38,9 @@
 //
 // Bound: the tensor pipe and the exponentials, each busy 56% of the time.
 // Measured (16/8 heads of 128, short bursts): 8192 tokens under a window of 4096
-// 182 us, 1130 TFLOP/s of visible work, 0.67 of the measured bf16 peak; 512 tokens
-// over 1100 visible rows 19 us; the prefix part of 64 sequences (32/8 heads) behind
+// 182-186 us, 1120 TFLOP/s of visible work, 0.66 of the measured bf16 peak; 512 tokens
+// over 1100 visible rows 19 us, 1 to 64 after 32700 rows 266 us (a CTA walks over all
+// keys of its tokens: 8 CTAs); the prefix part of 64 sequences (32/8 heads) behind
 // 32768 rows 40 us, 0.86 PFLOP/s.  A tile of two slots takes some 3150 clocks, of
 // which the tensor core works 2048 and a slot's exponentials 1400: with S, P and O
 // of two slots TMEM is full, and a slot's S waits for its P.V.

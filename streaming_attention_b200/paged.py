@@ -19,10 +19,10 @@ threads that call at once pass one each as ``ctx``.
 Workspaces come from torch's allocator: calls with different contexts, calls on
 different streams and calls captured into different graphs do not share one.
 
-A decode step of a small batch takes the GPU some ten microseconds, so the
-wrappers are written to cost the host less than that: one look at each
-tensor's layout, the cache description packed in one go, workspace sizes kept
-by shape.
+A call costs the host 11 to 17 us, as much as or more than a small batch's step
+takes the GPU, so the wrappers do little: one look at each tensor's layout, the
+cache description packed in one go, workspace sizes kept by shape.  A captured
+step leaves the host's part out.
 """
 from __future__ import annotations
 
