@@ -390,7 +390,9 @@ int sa_attn_decode_noalloc(void* stream, int dtype, const void* q, const void* k
  * and the partial sums.  Beyond, a result may be infinite or NaN.
  *
  * Workspaces are the caller's (256-byte aligned device memory); calls that may
- * run at the same time, captured ones included, need workspaces of their own.
+ * run at the same time, captured ones included, need workspaces of their own,
+ * and so do calls that several threads make at once on one stream (a call may
+ * be several launches).
  * Their sizes depend on the shapes in kv, on hq and on the prefix's length, not
  * on the sequences'.  A workspace's first SA_PAGED_ZERO_BYTES are zeros before
  * its first use, and every call, of either kind and any shape, leaves them zero
